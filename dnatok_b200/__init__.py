@@ -4,7 +4,8 @@ only implementation of the encode path."""
 from .tables import TokenizerSpec, Specials, UnsupportedTokenizer, spec_from_tokenizer, bpe_spec_from_json
 
 __all__ = ["B200Tokenizer", "GPUTokBPEBackend", "DnatokBpeKernel", "TokenizerSpec", "Specials",
-           "UnsupportedTokenizer", "spec_from_tokenizer", "bpe_spec_from_json"]
+           "UnsupportedTokenizer", "spec_from_tokenizer", "bpe_spec_from_json", "Automaton", "Grammar", "TokenHistory",
+           "process_logits", "process_logits_backward"]
 
 
 def __getattr__(name):
@@ -14,4 +15,10 @@ def __getattr__(name):
     if name in ("GPUTokBPEBackend", "DnatokBpeKernel"):
         from . import gputok_bpe_backend
         return getattr(gputok_bpe_backend, name)
+    if name == "Automaton":
+        from .automaton import Automaton
+        return Automaton
+    if name in ("Grammar", "TokenHistory", "process_logits", "process_logits_backward"):
+        from . import generate
+        return getattr(generate, name)
     raise AttributeError(name)

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "csrc", "libdnatok_b200.so")
@@ -24,7 +24,9 @@ EXPORTS = (
     "dnatok_scan_lengths", "dnatok_encode_host", "dnatok_launch_count", "dnatok_host_copy_bytes",
     "dnatok_encode_bpe_builtin_scratch", "dnatok_set_option", "dnatok_set_row_bytes_hint",
     "dnatok_pack_fasta", "dnatok_embed", "dnatok_create_kmer_table", "dnatok_set_start_lut",
-    "dnatok_row_summary", "dnatok_offset_bounds",
+    "dnatok_row_summary", "dnatok_offset_bounds", "dnatok_process_logits", "dnatok_process_logits_backward",
+    "dnatok_logits_scratch_bytes", "dnatok_history_add", "dnatok_create_grammar", "dnatok_destroy_grammar",
+    "dnatok_grammar_allowed", "dnatok_grammar_step",
 )
 BUILTIN_SCRATCH_BYTES = 8 << 20
 
@@ -36,6 +38,25 @@ class Specials(Structure):
 class Format(Structure):
     _fields_ = [("id_bits", c_int32), ("mask_bits", c_int32), ("add_special", c_int32),
                 ("pad_left", c_int32), ("max_tokens", c_int64), ("out_stride", c_int64)]
+
+
+F32, F16, BF16 = 0, 1, 2
+STATE_DEAD, STATE_FINISHED = -1, -2
+
+
+class Logits(Structure):
+    _fields_ = [("logits", c_void_p), ("dtype", c_int32), ("rows_bits", c_int32), ("n_rows", c_int64), ("width", c_int64),
+                ("stride", c_int64), ("seen", c_void_p), ("counts", c_void_p), ("history_rows", c_int64), ("rows", c_void_p),
+                ("repetition", c_float), ("frequency", c_float), ("presence", c_float), ("d_repetition", c_void_p),
+                ("d_frequency", c_void_p), ("d_presence", c_void_p), ("bias", c_void_p), ("bias_stride", c_int64),
+                ("allowed", c_void_p), ("allowed_stride", c_int64)]
+
+
+class History(Structure):
+    _fields_ = [("seen", c_void_p), ("counts", c_void_p), ("history_rows", c_int64), ("width", c_int64), ("ids", c_void_p),
+                ("id_bits", c_int32), ("rows_bits", c_int32), ("n_rows", c_int64), ("columns", c_int64),
+                ("id_stride", c_int64), ("lengths", c_void_p), ("pad_left", c_int32), ("offsets", c_void_p),
+                ("total", c_int64), ("rows", c_void_p)]
 
 
 class DnatokError(RuntimeError):
@@ -87,6 +108,16 @@ def lib() -> ctypes.CDLL:
     L.dnatok_offset_bounds.argtypes = [p, c_int64, p, p]
     L.dnatok_encode_host.argtypes = [p, c_int, p, p, c_int64, POINTER(Format), p, c_int64, p, p, p, p,
                                      POINTER(c_int64)]
+    L.dnatok_process_logits.argtypes = [POINTER(Logits), p, c_int32, c_int64, p]
+    L.dnatok_logits_scratch_bytes.argtypes = [c_int64, c_int64]
+    L.dnatok_logits_scratch_bytes.restype = c_size_t
+    L.dnatok_process_logits_backward.argtypes = [POINTER(Logits), p, c_int32, c_int64, p, c_int64, p, p, c_size_t, p]
+    L.dnatok_history_add.argtypes = [POINTER(History), c_int32, p]
+    L.dnatok_create_grammar.argtypes = [p, c_int32, c_int32, p, p, p, p, c_int64, c_int64, POINTER(p)]
+    L.dnatok_destroy_grammar.argtypes = [p]
+    L.dnatok_destroy_grammar.restype = None
+    L.dnatok_grammar_allowed.argtypes = [p, p, c_int64, p, p]
+    L.dnatok_grammar_step.argtypes = [p, p, p, c_int32, c_int64, p, p, p]
     if L.dnatok_version() != 1:
         raise RuntimeError("libdnatok_b200.so has ABI version %d, expected 1" % L.dnatok_version())
     _LIB = L

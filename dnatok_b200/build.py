@@ -11,8 +11,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(CSRC, "libdnatok_b200.so")
-SOURCES = ["dnatok_abi.cu", "bpe_table.cc"]
+SOURCES = ["dnatok_abi.cu", "generate_abi.cu", "bpe_table.cc"]
 DEPS = SOURCES + ["common.cuh", "emit_kernel.cuh", "embed_kernel.cuh", "kmer_kernel.cuh", "kmer_table_kernel.cuh", "bpe_kernel.cuh", "bpe_table.h",
+                  "abi_shared.h", "logits_kernel.cuh", "history_kernel.cuh", "grammar_kernel.cuh",
                   os.path.join("..", "..", "include", "dnatok_b200.h")]
 
 

@@ -18,6 +18,7 @@
 #include <thread>
 #include <vector>
 
+#include "abi_shared.h"
 #include "bpe_kernel.cuh"
 #include "bpe_table.h"
 #include "embed_kernel.cuh"
@@ -59,6 +60,20 @@ int fail(int code, const char* fmt, ...) {
     g_err = buf;
     return code;
 }
+
+}  // namespace
+
+int dnatok::abi_fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+void dnatok::abi_count_launch() { ++g_launches; }
+
+namespace {
 
 #define CUDA_TRY(expr)                                                                          \
     do {                                                                                        \

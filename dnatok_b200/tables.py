@@ -454,3 +454,49 @@ def spec_from_tokenizer(tok: Any) -> TokenizerSpec:
             raise UnsupportedTokenizer("unk id mismatch between tokenizer and tokenizer.json")
         return spec
     return spec_from_probing(tok)
+
+
+# --------------------------------------------------------------------------- the bytes of every token
+
+def token_bytes(spec: TokenizerSpec) -> List[bytes]:
+    """The text every id stands for (empty: a special, the unknown id or an id without one), from the tables the kernels
+    encode with.  Where several bytes give one id (soft-masked letters, say) it is the upper-case one."""
+    sp = spec.specials
+    special = {sp.pad_id, sp.unk_id, sp.cls_id, sp.sep_id}
+    luts = [np.asarray(spec.lut256)] + ([np.asarray(spec.start_lut256)] if spec.start_lut256 is not None else [])
+    tops = [int(a.max()) for a in luts + [np.asarray(x) for x in (spec.kmer_ids, spec.kmer_table5, spec.merge_out) if x is not None and len(x)]]
+    text = [b""] * max([spec.vocab_size] + [t + 1 for t in tops])
+
+    def put(i: int, b: bytes) -> None:
+        if i >= 0 and i not in special and not text[i]:
+            text[i] = b
+
+    upper_first = sorted(range(256), key=lambda c: (not 65 <= c <= 90, c))
+    for lut in luts:
+        for c in upper_first:
+            put(int(lut[c]), bytes([c]))
+    if spec.kind == "kmer":
+        singles = {int(i) for i in luts[0]}
+        if spec.kmer_ids is not None:
+            for w, i in zip(itertools.product(b"ACGT", repeat=spec.k), np.asarray(spec.kmer_ids).tolist()):
+                if i not in singles:
+                    put(i, bytes(w))
+        if spec.kmer_table5 is not None:
+            table = np.asarray(spec.kmer_table5).tolist()
+            windows = list(zip(itertools.product(b"ACGTN", repeat=spec.k), table))
+            for w, i in [x for x in windows if ord("N") not in x[0]] + [x for x in windows if ord("N") in x[0]]:
+                if i not in singles:
+                    put(i, bytes(w))
+    if spec.kind == "bpe":
+        left = list(zip(np.asarray(spec.merge_a).tolist(), np.asarray(spec.merge_b).tolist(), np.asarray(spec.merge_out).tolist()))
+        while left:                                  # (an operand may be created by a later merge)
+            wait = []
+            for a, b, o in left:
+                if text[a] and text[b]:
+                    put(o, text[a] + text[b])
+                else:
+                    wait.append((a, b, o))
+            if len(wait) == len(left):
+                break
+            left = wait
+    return text

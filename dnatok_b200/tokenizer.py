@@ -304,6 +304,24 @@ class B200Tokenizer:
             lengths.zero_()
         return BatchEncoding(embeddings=out, lengths=lengths[:B])
 
+    # ------------------------------------------------------------------ generation over this vocabulary
+    def token_history(self, n_rows: int, *, width: Optional[int] = None, counts: bool = True):
+        """An empty ``TokenHistory`` of ``n_rows`` rows over this vocabulary, for ``process_logits``; ``width``: columns of the
+        logits where they have more than the vocabulary."""
+        from .generate import TokenHistory
+        width = self.vocab_size if width is None else int(width)
+        if width < self.vocab_size:
+            raise ValueError("width %d is smaller than the vocabulary (%d tokens)" % (width, self.vocab_size))
+        return TokenHistory(n_rows, width, device=self.device, counts=counts)
+
+    def grammar(self, automaton, *, width: Optional[int] = None):
+        """A ``Grammar``: what the automaton allows of this vocabulary.  The separator ends a row; other specials and the
+        unknown token never follow."""
+        from .generate import Grammar
+        from .tables import token_bytes
+        sep = self.spec.specials.sep_id
+        return Grammar(automaton, token_bytes(self.spec), end_id=sep if sep >= 0 else None, width=width)
+
     def _raise_on_status(self, status, truncation: bool) -> None:
         bits = int(status.max().item()) if status.numel() else 0
         if not bits:

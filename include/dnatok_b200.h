@@ -278,6 +278,96 @@ int dnatok_pack_fasta(const char* text, int64_t n_text, uint8_t* out_bytes, int6
  *                           warps, larger ones a warp per word; -1 (default): the automatic choice above */
 int dnatok_set_option(const char* name, int64_t value);
 
+/* ---- between a model's logits and the choice of its next token (no reference counterpart) ----
+ *
+ * Sets of tokens are words of 32 bits, (width + 31) / 32 of them: bit v % 32 of word v / 32 stands for token v.  width is
+ * the number of columns of the logits; it may exceed the vocabulary.  Device buffers are the caller's; a grammar owns
+ * its tables (uploaded once per device on first use, which has to be outside of stream capture). */
+
+#define DNATOK_F32  0
+#define DNATOK_F16  1
+#define DNATOK_BF16 2
+
+#define DNATOK_STATE_DEAD     (-1)    /* a token that was not allowed was taken: nothing may follow */
+#define DNATOK_STATE_FINISHED (-2)    /* after the end token: only the end token may follow */
+
+typedef struct {
+    const void* logits;               /* [n_rows, width], `stride` elements from row to row (0 and up) */
+    int32_t dtype;                    /* DNATOK_F32, DNATOK_F16 or DNATOK_BF16 */
+    int32_t rows_bits;                /* type of `rows`: 32 or 64 */
+    int64_t n_rows, width, stride;
+    const uint32_t* seen;             /* [history_rows, words] tokens a row has seen; NULL: none */
+    const int32_t* counts;            /* [history_rows, width] how often it generated each; NULL: never */
+    int64_t history_rows;
+    const void* rows;                 /* [n_rows] history row of each logits row (one outside the history: no history);
+                                         NULL: the same, and history_rows must be n_rows */
+    float repetition, frequency, presence;            /* one number for all rows ... */
+    const float *d_repetition, *d_frequency, *d_presence;   /* ... or [n_rows] on the device, where not NULL */
+    const float* bias;                /* [width] (bias_stride 0) or [n_rows, width]; NULL: none */
+    int64_t bias_stride;
+    const uint32_t* allowed;          /* [words] (allowed_stride 0) or [n_rows, words]; NULL: all are allowed */
+    int64_t allowed_stride;
+} dnatok_logits;
+
+/* out = allowed ? x2 + bias : -inf, where a token that the row has seen has x1 = x > 0 ? x / repetition : x * repetition
+ * and one that it generated c > 0 times x2 = x1 - frequency * c - presence; other tokens keep x.  Computed in 32 bits,
+ * rounded once to the output's type: that of the logits or DNATOK_F32.  Logits that are not allowed have no influence, NaN
+ * included; a row without an allowed token is -inf throughout.  d_out may be the logits themselves (same type and stride);
+ * another overlap is not allowed. */
+int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtype, int64_t out_stride, dnatok_stream stream);
+
+/* Bytes of 256-byte aligned device scratch that dnatok_process_logits_backward needs for a shared bias' gradient. */
+size_t dnatok_logits_scratch_bytes(int64_t n_rows, int64_t width);
+
+/* The gradient of dnatok_process_logits for d_grad (the gradient of its output; the output's type): d_dlogits (the
+ * logits' type; NULL: not wanted) and d_dbias (float, [width] where bias_stride is 0, else [n_rows, width] contiguous;
+ * NULL: not wanted).  in->bias and in->counts are not read.  A shared bias' gradient is summed in 32 bits in an order
+ * that depends on the sizes only.  d_dlogits may be d_grad itself where type and stride are the same. */
+int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, int32_t grad_dtype, int64_t grad_stride,
+                                   void* d_dlogits, int64_t dlogits_stride, float* d_dbias, void* d_scratch,
+                                   size_t scratch_bytes, dnatok_stream stream);
+
+typedef struct {
+    uint32_t* seen;                   /* [history_rows, words] */
+    int32_t* counts;                  /* [history_rows, width]; NULL: not kept */
+    int64_t history_rows, width;
+    const void* ids;
+    int32_t id_bits;                  /* 32 or 64 */
+    int32_t rows_bits;                /* type of `rows`: 32 or 64 */
+    int64_t n_rows;
+    int64_t columns, id_stride;       /* padded rows: ids a row, and from row to row */
+    const int32_t* lengths;           /* padded rows: [n_rows] ids of each; NULL: all columns */
+    int32_t pad_left;                 /* padded rows: 1 if the padding comes first */
+    const int64_t* offsets;           /* flat ids: [n_rows + 1], as dnatok_encode writes them; NULL: padded rows */
+    int64_t total;                    /* flat ids: how many */
+    const void* rows;                 /* [n_rows] history row of each row; NULL: the same, and history_rows must be n_rows */
+} dnatok_history;
+
+/* Every id of a row is entered in its history row: its bit in `seen`, and `counts` raised by one where generated != 0 and
+ * counts are kept.  Ids outside [0, width) are no tokens and rows outside the history take nothing; two rows may name one
+ * history row. */
+int dnatok_history_add(const dnatok_history* h, int32_t generated, dnatok_stream stream);
+
+typedef struct dnatok_grammar dnatok_grammar;
+
+/* A finite automaton over bytes and the bytes of every token.  next[state * n_classes + class] is the following state or
+ * -1; byte_class[256] names a byte's class (< n_classes); accepting[state] != 0: the row may end there.  Token v's bytes are
+ * token_bytes[token_offsets[v] .. token_offsets[v + 1]); one without bytes is never allowed, but for end_id (-1: none). */
+int dnatok_create_grammar(const int32_t* next, int32_t n_states, int32_t n_classes, const uint8_t* accepting,
+                          const uint8_t byte_class[256], const uint8_t* token_bytes, const int64_t* token_offsets,
+                          int64_t width, int64_t end_id, dnatok_grammar** out);
+void dnatok_destroy_grammar(dnatok_grammar* g);
+
+/* d_allowed[row] = the tokens whose bytes lead from d_states[row] to a live state; the end token where the state accepts
+ * or the row is finished.  A state outside the automaton allows nothing. */
+int dnatok_grammar_allowed(dnatok_grammar* g, const int32_t* d_states, int64_t n_rows, uint32_t* d_allowed,
+                           dnatok_stream stream);
+
+/* d_states_out[row] = the state after d_tokens[row] (token_bits 32 or 64); a token outside [0, width) leaves the row as it
+ * was.  With d_allowed, the masks of the new states too; d_states_out may then not be d_states. */
+int dnatok_grammar_step(dnatok_grammar* g, const int32_t* d_states, const void* d_tokens, int32_t token_bits, int64_t n_rows,
+                        int32_t* d_states_out, uint32_t* d_allowed, dnatok_stream stream);
+
 /* Number of kernels this library has launched from the calling process (for accounting). */
 int64_t dnatok_launch_count(void);
 
