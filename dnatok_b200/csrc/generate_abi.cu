@@ -1,10 +1,13 @@
 // C ABI of the operators between a model's logits and the choice of its next token (see include/dnatok_b200.h).
 #include "../../include/dnatok_b200.h"
 
+#include <algorithm>
 #include <climits>
+#include <cstring>
 #include <map>
 #include <mutex>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "abi_shared.h"
@@ -34,7 +37,8 @@ size_t size_of(int dtype) { return dtype == DNATOK_F32 ? 4 : 2; }
 bool known(int dtype) { return dtype == DNATOK_F32 || dtype == DNATOK_F16 || dtype == DNATOK_BF16; }
 
 // Blocks for `n` threads' worth of work in blocks of `threads`, at most what a grid-stride loop needs to fill the GPU.
-unsigned blocks_for(int64_t n, int threads, int64_t most = 148 * 16) {
+constexpr int SMS = 148;
+unsigned blocks_for(int64_t n, int threads, int64_t most = SMS * 16) {
     const int64_t b = (n + threads - 1) / threads;
     return (unsigned)(b < 1 ? 1 : b > most ? most : b);
 }
@@ -58,7 +62,7 @@ int check_logits(const dnatok_logits* in) {
     if (!aligned(in->logits, size_of(in->dtype))) return abi_fail(DNATOK_ERR_INVALID, "misaligned logits");
     if (in->counts && !in->seen) return abi_fail(DNATOK_ERR_INVALID, "counts without seen");
     if (in->seen) {
-        if (in->history_rows < 0) return abi_fail(DNATOK_ERR_INVALID, "history_rows < 0");
+        if (in->history_rows < 0 || in->history_rows > INT32_MAX) return abi_fail(DNATOK_ERR_INVALID, "bad number of history rows");
         if (int rc = check_rows(in->rows, in->rows_bits, in->n_rows, in->history_rows)) return rc;
     }
     const int64_t words = (in->width + 31) / 32;
@@ -66,14 +70,15 @@ int check_logits(const dnatok_logits* in) {
     if (in->allowed && in->allowed_stride != 0 && in->allowed_stride < words) return abi_fail(DNATOK_ERR_INVALID, "allowed_stride smaller than a row");
     const void* words32[] = {in->seen, in->counts, in->d_repetition, in->d_frequency, in->d_presence, in->bias, in->allowed};
     for (const void* p : words32) if (!aligned(p, 4)) return abi_fail(DNATOK_ERR_INVALID, "misaligned 32-bit array");
-    if (!in->d_repetition && !(in->repetition > 0.f)) return abi_fail(DNATOK_ERR_INVALID, "repetition must be positive");
+    if (!in->d_repetition && !(in->repetition >= 0x1p-126f && in->repetition <= 0x1p126f))      // (so that 1 / r is a normal number too)
+        return abi_fail(DNATOK_ERR_INVALID, "repetition must be positive and finite (2^-126 to 2^126)");
     return 0;
 }
 
 LogitsArgs logits_args(const dnatok_logits* in) {
     LogitsArgs a;
     a.n_rows = in->n_rows; a.width = in->width; a.stride = in->stride;
-    a.seen = in->seen; a.counts = in->counts; a.history_rows = in->history_rows;
+    a.seen = in->seen; a.counts = in->counts; a.history_rows = (int32_t)in->history_rows;
     a.rows = in->rows; a.rows_bits = in->rows_bits;
     a.repetition = in->repetition; a.frequency = in->frequency; a.presence = in->presence;
     a.d_repetition = in->d_repetition; a.d_frequency = in->d_frequency; a.d_presence = in->d_presence;
@@ -87,6 +92,36 @@ int check_output(const char* what, const void* p, size_t size, int64_t stride, c
     if (!aligned(p, size)) return abi_fail(DNATOK_ERR_INVALID, "misaligned %s", what);
     if (in->n_rows > 1 && stride < in->width) return abi_fail(DNATOK_ERR_INVALID, "rows of %s overlap", what);
     return 0;
+}
+
+// Whether rows of elements of `size` bytes can be moved 16 bytes at a time.  An array that is not there can.
+bool vector_rows(const void* p, int64_t stride, size_t size, int64_t n_rows) {
+    return !p || (aligned(p, 16) && (n_rows <= 1 || stride * (int64_t)size % 16 == 0));
+}
+
+int64_t rows_per_block(int64_t n_rows, int64_t groups) {
+    const int64_t per_warp = (n_rows + groups * LOGITS_WARPS - 1) / (groups * LOGITS_WARPS);
+    return per_warp * LOGITS_WARPS;
+}
+
+// A block for every tile of columns and group of rows.  Each warp gets one row where there are few blocks, then as many
+// rows as leave about 16 blocks an SM: their loads of what belongs to the columns, and the partial sums of a bias' gradient,
+// are spread over those rows.
+dim3 logits_grid(int64_t n_rows, int64_t width) {
+    const int64_t tiles = (width + LOGITS_TILE - 1) / LOGITS_TILE;
+    int64_t groups = ((int64_t)SMS * 16 + tiles - 1) / tiles;
+    const int64_t most = (n_rows + LOGITS_WARPS - 1) / LOGITS_WARPS;
+    if (groups > most) groups = most;
+    const int64_t rows = rows_per_block(n_rows, groups);
+    return dim3((unsigned)tiles, (unsigned)((n_rows + rows - 1) / rows));
+}
+
+// Which columns a lane takes (see logits_kernel.cuh).
+template <size_t S, size_t U, typename F>
+void with_map(bool vector, int64_t width, F f) {
+    constexpr int MAP = (S > 2 || U > 2) ? HALVES : CONTIGUOUS;
+    if (!vector || width % (MAP == HALVES ? 4 : 8)) f(std::integral_constant<int, APART>());
+    else f(std::integral_constant<int, MAP>());
 }
 
 // Calls f with a null pointer of the element type.
@@ -110,19 +145,29 @@ int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtyp
     if (in->n_rows == 0) return DNATOK_OK;
     cudaStream_t st = (cudaStream_t)stream;
     const LogitsArgs a = logits_args(in);
-    const unsigned grid = blocks_for(a.n_rows * a.width, LOGITS_THREADS);
+    const bool vector = vector_rows(in->logits, in->stride, size_of(in->dtype), in->n_rows) &&
+                        vector_rows(d_out, out_stride, size_of(out_dtype), in->n_rows) &&
+                        vector_rows(in->bias, in->bias_stride, 4, in->n_rows);
+    const int64_t groups = (a.n_rows + LOGITS_WARPS - 1) / LOGITS_WARPS;
+    const dim3 grid((unsigned)((a.width + LOGITS_TILE - 1) / LOGITS_TILE), (unsigned)(groups < 65535 ? groups : 65535));
     with_type(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (out_dtype == in->dtype) process_logits_kernel<T, T><<<grid, LOGITS_THREADS, 0, st>>>(a, (const T*)in->logits, (T*)d_out, out_stride);
-        else process_logits_kernel<T, float><<<grid, LOGITS_THREADS, 0, st>>>(a, (const T*)in->logits, (float*)d_out, out_stride);
+        auto typed = [&](auto* o) {
+            using O = std::remove_pointer_t<decltype(o)>;
+            with_map<sizeof(T), sizeof(O)>(vector, a.width, [&](auto m) {
+                process_logits_kernel<T, O, decltype(m)::value><<<grid, LOGITS_THREADS, 0, st>>>(a, (const T*)in->logits, (O*)d_out, out_stride);
+            });
+        };
+        if (out_dtype == in->dtype) typed(t); else typed((float*)nullptr);
     });
     LAUNCH_CHECK("process_logits_kernel");
     return DNATOK_OK;
 }
 
 size_t dnatok_logits_scratch_bytes(int64_t n_rows, int64_t width) {
-    (void)n_rows; (void)width;
-    return 0;
+    if (n_rows < 1 || width < 1) return 0;
+    const unsigned blocks = logits_grid(n_rows, width).y;
+    return blocks > 1 ? (size_t)blocks * (size_t)width * 4 : 0;
 }
 
 int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, int32_t grad_dtype, int64_t grad_stride,
@@ -136,35 +181,98 @@ int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, 
     if (d_dlogits) if (int rc = check_output("logits' gradient", d_dlogits, size_of(in->dtype), dlogits_stride, in)) return rc;
     if (d_dlogits && d_dlogits == d_grad && in->n_rows && (grad_dtype != in->dtype || (in->n_rows > 1 && grad_stride != dlogits_stride)))
         return abi_fail(DNATOK_ERR_INVALID, "in place both gradients have one type and stride");
-    (void)d_scratch; (void)scratch_bytes;
     cudaStream_t st = (cudaStream_t)stream;
     const bool shared = in->bias_stride == 0;
     if (in->n_rows == 0) {
         if (d_dbias && shared) CUDA_TRY(cudaMemsetAsync(d_dbias, 0, (size_t)in->width * 4, st));
         return DNATOK_OK;
     }
+    if (!d_dlogits && !d_dbias) return DNATOK_OK;
     const LogitsArgs a = logits_args(in);
-    auto run = [&](auto* t, auto* g) -> int {
+    const bool vector = vector_rows(in->logits, in->stride, size_of(in->dtype), in->n_rows) &&
+                        vector_rows(d_grad, grad_stride, size_of(grad_dtype), in->n_rows) &&
+                        vector_rows(d_dlogits, dlogits_stride, size_of(in->dtype), in->n_rows) &&
+                        (shared || vector_rows(d_dbias, in->width, 4, in->n_rows));
+    const dim3 grid = logits_grid(a.n_rows, a.width);
+    const int rows = (int)rows_per_block(a.n_rows, grid.y);
+    const bool join = d_dbias && shared && grid.y > 1;
+    if (join && (!d_scratch || scratch_bytes < dnatok_logits_scratch_bytes(a.n_rows, a.width) || !aligned(d_scratch, 256)))
+        return abi_fail(DNATOK_ERR_SCRATCH, "the gradient of a shared bias needs %zu bytes of 256-byte aligned scratch",
+                        dnatok_logits_scratch_bytes(a.n_rows, a.width));
+    float* sums = join ? (float*)d_scratch : d_dbias;
+    with_type(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        using G = std::remove_pointer_t<decltype(g)>;
-        if (d_dbias && shared) {       // before the logits' gradient, which may overwrite the gradient
-            bias_gradient_kernel<G><<<(unsigned)((a.width + LOGITS_THREADS - 1) / LOGITS_THREADS), LOGITS_THREADS, 0, st>>>(
-                a, (const G*)d_grad, grad_stride, d_dbias);
-            LAUNCH_CHECK("bias_gradient_kernel");
-        }
-        if (d_dlogits || (d_dbias && !shared)) {
-            logits_gradient_kernel<T, G><<<blocks_for(a.n_rows * a.width, LOGITS_THREADS), LOGITS_THREADS, 0, st>>>(
-                a, (const T*)in->logits, (const G*)d_grad, grad_stride, (T*)d_dlogits, dlogits_stride, shared ? nullptr : d_dbias);
-            LAUNCH_CHECK("logits_gradient_kernel");
-        }
-        return DNATOK_OK;
-    };
-    int rc = DNATOK_OK;
-    with_type(in->dtype, [&](auto* t) { rc = grad_dtype == in->dtype ? run(t, t) : run(t, (float*)nullptr); });
-    return rc;
+        auto typed = [&](auto* g) {
+            using G = std::remove_pointer_t<decltype(g)>;
+            with_map<sizeof(T), sizeof(G)>(vector, a.width, [&](auto m) {
+                constexpr int MAP = decltype(m)::value;
+                if (d_dbias && shared)
+                    logits_gradient_kernel<T, G, MAP, true><<<grid, LOGITS_THREADS, 0, st>>>(
+                        a, (const T*)in->logits, (const G*)d_grad, grad_stride, (T*)d_dlogits, dlogits_stride, sums, rows);
+                else
+                    logits_gradient_kernel<T, G, MAP, false><<<grid, LOGITS_THREADS, 0, st>>>(
+                        a, (const T*)in->logits, (const G*)d_grad, grad_stride, (T*)d_dlogits, dlogits_stride, d_dbias, rows);
+            });
+        };
+        if (grad_dtype == in->dtype) typed(t); else typed((float*)nullptr);
+    });
+    LAUNCH_CHECK("logits_gradient_kernel");
+    if (join) {
+        bias_gradient_kernel<<<(unsigned)((a.width + LOGITS_THREADS - 1) / LOGITS_THREADS), LOGITS_THREADS, 0, st>>>(sums, (int)grid.y, a.width, d_dbias);
+        LAUNCH_CHECK("bias_gradient_kernel");
+    }
+    return DNATOK_OK;
 }
 
+}  // extern "C"
+
 // ------------------------------------------------------------------ history
+
+namespace {
+
+template <typename IdT>
+int launch_history(const HistoryArgs& a, const IdT* ids, cudaStream_t st) {
+    const int64_t mean = a.offsets ? a.total / a.n_rows : a.columns;     // ids a row, as far as the host knows
+    // A row with at least as many ids as there are tokens is counted in shared memory first (8 x 1,048,576 ids of bytes:
+    // 16 us; entered one by one they queue up at ten counters a row: 10,800 us).  A row that is only marked needs 32
+    // times less to clear and to join.
+    const int64_t words = (a.width + 31) / 32, table = a.counts ? a.width : words;
+    if (mean >= 1024 && mean >= (a.counts ? table : 4 * table) && table * 4 <= 192 * 1024 && a.n_rows <= (1 << 20)) {
+        int64_t splits = ((int64_t)SMS * 3 + a.n_rows - 1) / a.n_rows;
+        const int64_t least = table > 1024 ? table : 1024;                // ids a block
+        if (splits > mean / least) splits = mean / least;
+        if (splits < 1) splits = 1;
+        int log_copies = 0;
+        while (a.counts && log_copies < 5 && (table << (log_copies + 1)) * 4 <= 64 * 1024 && (table << (log_copies + 1)) <= mean / splits) ++log_copies;
+        const size_t shared = (size_t)(table << log_copies) * 4;
+        const unsigned grid = (unsigned)(a.n_rows * splits);
+        if (a.counts) {
+            if (shared > 48 * 1024) CUDA_TRY(cudaFuncSetAttribute(history_count_kernel<IdT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024));
+            history_count_kernel<IdT><<<grid, HISTORY_LONG_THREADS, shared, st>>>(a, ids, (int)splits, log_copies);
+            LAUNCH_CHECK("history_count_kernel");
+        } else {
+            if (shared > 48 * 1024) CUDA_TRY(cudaFuncSetAttribute(history_mark_kernel<IdT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024));
+            history_mark_kernel<IdT><<<grid, HISTORY_LONG_THREADS, shared, st>>>(a, ids, (int)splits);
+            LAUNCH_CHECK("history_mark_kernel");
+        }
+        return DNATOK_OK;
+    }
+    int group = 1;                                                        // threads a row: about one for four ids
+    while (group < HISTORY_THREADS && group * 4 < mean) group *= 2;
+    int64_t splits = (mean + group * 8 - 1) / (group * 8);
+    const int64_t most = (int64_t)SMS * 2048 / group / a.n_rows;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    const int64_t blocks = (a.n_rows * splits * group + HISTORY_THREADS - 1) / HISTORY_THREADS;
+    if (blocks > INT32_MAX) return abi_fail(DNATOK_ERR_UNSUPPORTED, "too many rows for one call");
+    history_add_kernel<IdT><<<(unsigned)blocks, HISTORY_THREADS, 0, st>>>(a, ids, group, (int)splits);
+    LAUNCH_CHECK("history_add_kernel");
+    return DNATOK_OK;
+}
+
+}  // namespace
+
+extern "C" {
 
 int dnatok_history_add(const dnatok_history* h, int32_t generated, dnatok_stream stream) {
     if (!h) return abi_fail(DNATOK_ERR_INVALID, "NULL argument");
@@ -183,11 +291,7 @@ int dnatok_history_add(const dnatok_history* h, int32_t generated, dnatok_stream
     a.offsets = h->offsets; a.total = h->total; a.lengths = h->lengths; a.pad_left = h->pad_left;
     a.rows = h->rows; a.rows_bits = h->rows_bits;
     cudaStream_t st = (cudaStream_t)stream;
-    const unsigned grid = blocks_for(a.n_rows * 32, HISTORY_THREADS);
-    if (h->id_bits == 64) history_add_kernel<int64_t><<<grid, HISTORY_THREADS, 0, st>>>(a, (const int64_t*)h->ids);
-    else history_add_kernel<int32_t><<<grid, HISTORY_THREADS, 0, st>>>(a, (const int32_t*)h->ids);
-    LAUNCH_CHECK("history_add_kernel");
-    return DNATOK_OK;
+    return h->id_bits == 64 ? launch_history(a, (const int64_t*)h->ids, st) : launch_history(a, (const int32_t*)h->ids, st);
 }
 
 }  // extern "C"
@@ -196,9 +300,15 @@ int dnatok_history_add(const dnatok_history* h, int32_t generated, dnatok_stream
 
 struct dnatok_grammar {
     std::vector<int32_t> next;
+    std::vector<uint16_t> step16;
+    std::vector<uint32_t> step32;
     std::vector<uint8_t> accepting, codes;
     std::vector<int32_t> token_at;
-    int32_t n_states = 0, n_classes = 0;
+    std::vector<uint64_t> text;
+    std::vector<uint32_t> super;
+    std::vector<uint2> prefix;
+    std::vector<uint4> rest;
+    int32_t n_states = 0, log_pitch = 0, n_groups = 0, super_steps = 0, prefix_steps = 0;
     int64_t width = 0, end_id = -1;
     struct Device { void* memory = nullptr; GrammarTables tables{}; };
     std::mutex mu;
@@ -220,28 +330,40 @@ int grammar_tables(dnatok_grammar* g, cudaStream_t stream, GrammarTables* out) {
         CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
         if (capturing != cudaStreamCaptureStatusNone)
             return abi_fail(DNATOK_ERR_INVALID, "a grammar's first use on a device must be outside of stream capture");
-        const size_t sizes[4] = {g->next.size() * 4, g->accepting.size(), g->codes.size(), g->token_at.size() * 4};
-        const void* from[4] = {g->next.data(), g->accepting.data(), g->codes.data(), g->token_at.data()};
-        size_t at[5] = {0};
-        for (int i = 0; i < 4; ++i) at[i + 1] = at[i] + up256(sizes[i] + 1);
+        constexpr int N = 10;
+        const size_t sizes[N] = {g->next.size() * 4, g->step16.size() * 2, g->accepting.size(), g->codes.size(), g->token_at.size() * 4,
+                                 g->text.size() * 8, g->prefix.size() * 8, g->rest.size() * 16, g->step32.size() * 4, g->super.size() * 4};
+        const void* from[N] = {g->next.data(), g->step16.data(), g->accepting.data(), g->codes.data(), g->token_at.data(),
+                               g->text.data(), g->prefix.data(), g->rest.data(), g->step32.data(), g->super.data()};
+        size_t at[N + 1] = {0};
+        for (int i = 0; i < N; ++i) at[i + 1] = at[i] + up256(sizes[i] + 1);
         struct Undo {
             void* memory = nullptr;
             cudaStream_t copies = nullptr;
             ~Undo() { if (copies) cudaStreamDestroy(copies); if (memory) cudaFree(memory); }
         } undo;
-        CUDA_TRY(cudaMalloc(&undo.memory, at[4]));
+        CUDA_TRY(cudaMalloc(&undo.memory, at[N]));
         CUDA_TRY(cudaStreamCreateWithFlags(&undo.copies, cudaStreamNonBlocking));
         char* base = (char*)undo.memory;
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < N; ++i)
             if (sizes[i]) CUDA_TRY(cudaMemcpyAsync(base + at[i], from[i], sizes[i], cudaMemcpyHostToDevice, undo.copies));
         CUDA_TRY(cudaStreamSynchronize(undo.copies));
         dnatok_grammar::Device d;
         GrammarTables& t = d.tables;
         t.next = (const int32_t*)(base + at[0]);
-        t.accepting = (const uint8_t*)(base + at[1]);
-        t.codes = (const uint8_t*)(base + at[2]);
-        t.token_at = (const int32_t*)(base + at[3]);
-        t.n_states = g->n_states; t.n_classes = g->n_classes; t.width = g->width; t.end_id = g->end_id;
+        t.step16 = g->step16.empty() ? nullptr : (const uint16_t*)(base + at[1]);
+        t.step32 = (const uint32_t*)(base + at[8]);
+        t.accepting = (const uint8_t*)(base + at[2]);
+        t.codes = (const uint8_t*)(base + at[3]);
+        t.token_at = (const int32_t*)(base + at[4]);
+        t.text = g->text.empty() ? nullptr : (const uint64_t*)(base + at[5]);
+        t.prefix = (const uint2*)(base + at[6]);
+        t.super = (const uint32_t*)(base + at[9]);
+        t.rest = (const uint4*)(base + at[7]);
+        t.n_states = g->n_states; t.log_pitch = g->log_pitch; t.n_groups = g->n_groups;
+        t.n_super = (int32_t)g->super.size();
+        t.super_steps = g->super_steps; t.prefix_steps = g->prefix_steps;
+        t.width = g->width; t.end_id = g->end_id;
         d.memory = undo.memory;
         it = g->dev.emplace(dev, d).first;
         undo.memory = nullptr;
@@ -256,10 +378,127 @@ int check_states(const dnatok_grammar* g, const void* states, int64_t n_rows) {
     return 0;
 }
 
-int launch_allowed(const GrammarTables& t, const int32_t* states, int64_t n_rows, uint32_t* allowed, cudaStream_t st) {
-    grammar_allowed_kernel<<<blocks_for(n_rows * ((t.width + 31) / 32) * 32, GRAMMAR_THREADS), GRAMMAR_THREADS, 0, st>>>(t, states, n_rows, allowed);
+// With tokens: the states are advanced first.
+int launch_allowed(const GrammarTables& t, const int32_t* states, const void* tokens, int token_bits, int32_t* states_out, int64_t n_rows,
+                   uint32_t* allowed, cudaStream_t st) {
+    const int64_t words = (t.width + 31) / 32;
+    // The sorted groups need a row's words in shared memory; vocabularies beyond 262,144 tokens and automata with more than
+    // 15 classes go token by token.
+    if (!t.text || words > 8192 || n_rows > INT32_MAX / 8) {
+        if (tokens) {
+            grammar_advance_kernel<<<(unsigned)((n_rows + GRAMMAR_THREADS - 1) / GRAMMAR_THREADS), GRAMMAR_THREADS, 0, st>>>(
+                t, states, tokens, token_bits, n_rows, states_out);
+            LAUNCH_CHECK("grammar_advance_kernel");
+            states = states_out;
+        }
+        grammar_any_kernel<<<blocks_for(n_rows * words * 32, GRAMMAR_THREADS), GRAMMAR_THREADS, 0, st>>>(t, states, n_rows, allowed);
+        LAUNCH_CHECK("grammar_any_kernel");
+        return DNATOK_OK;
+    }
+    // A warp for every 4 groups, up to 8 where rows fill the GPU, else up to 16.  Few rows: up to 8 blocks a row, as long as
+    // all are on the GPU at once and each of their warps has 4 groups.
+    int parts = 1;
+    while (parts < 8 && n_rows * parts * 2 <= SMS * 4 && t.n_groups > parts * 128) parts *= 2;
+    int warps = 1;
+    const int most = n_rows > SMS * 4 ? 8 : GRAMMAR_MOST / 32;
+    while (warps < most && warps * 4 * parts < t.n_groups) warps *= 2;
+    int split = 1;                                            // warps a set of 32 groups
+    while (split < 32 && split < warps * parts && t.n_super * split < warps * parts) split *= 2;
+    const size_t table = (((size_t)(t.n_states + 1) << t.log_pitch) * (t.step16 ? 2 : 4) + 15) / 16 * 16;
+    const bool near = table <= GRAMMAR_NEAR_BYTES;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n_rows * parts));
+    cfg.blockDim = dim3((unsigned)warps * 32);
+    cfg.dynamicSmemBytes = (near ? table : 0) + (size_t)words * 4;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)parts; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    cudaError_t e = cudaSuccess;
+    auto run = [&](auto s, auto n, auto c) {
+        e = cudaLaunchKernelEx(&cfg, grammar_allowed_kernel<decltype(s), decltype(n)::value, decltype(c)::value>, t, states, tokens,
+                               token_bits, states_out, allowed, parts, split);
+    };
+    auto placed = [&](auto s, auto n) { if (parts > 1) run(s, n, std::true_type()); else run(s, n, std::false_type()); };
+    auto typed = [&](auto s) { if (near) placed(s, std::true_type()); else placed(s, std::false_type()); };
+    if (t.step16) typed(uint16_t()); else typed(uint32_t());
+    if (e != cudaSuccess) return abi_fail(DNATOK_ERR_CUDA, "launch of grammar_allowed_kernel: %s", cudaGetErrorString(e));
     LAUNCH_CHECK("grammar_allowed_kernel");
     return DNATOK_OK;
+}
+
+// The tokens in the order of their groups (see grammar_kernel.cuh): what a group shares, what each has behind it, who it is.
+void sort_tokens(dnatok_grammar* g) {
+    auto code = [&](int32_t v, int64_t i) { return g->codes[(size_t)(g->token_at[(size_t)v] + i)]; };
+    auto length = [&](int32_t v) { return (int64_t)g->token_at[(size_t)v + 1] - g->token_at[(size_t)v]; };
+    auto classes = [&](int32_t v, int64_t from, int64_t to, int64_t filled) {
+        uint64_t p = 0;
+        for (int64_t i = 0; i < filled; ++i)
+            p |= (uint64_t)(from + i < to ? code(v, from + i) : (1 << g->log_pitch) - 1) << (4 * i);
+        return p;
+    };
+    std::vector<int32_t> order;
+    g->text.assign((size_t)g->width, 0);
+    for (int32_t v = 0; v < g->width; ++v) {
+        const int64_t n = length(v);
+        g->text[(size_t)v] = n > GRAMMAR_PACKED ? 15ull << 60 : (uint64_t)n << 60 | classes(v, 0, n, n);
+        if (length(v) && v != g->end_id) order.push_back(v);
+    }
+    const int64_t mean = order.empty() ? 0 : ((int64_t)g->codes.size() + (int64_t)order.size() - 1) / (int64_t)order.size();
+    std::sort(order.begin(), order.end(), [&](int32_t x, int32_t y) {
+        if ((length(x) > mean) != (length(y) > mean)) return length(y) > mean;
+        const int64_t n = std::min(length(x), length(y));
+        const int c = memcmp(&g->codes[(size_t)g->token_at[(size_t)x]], &g->codes[(size_t)g->token_at[(size_t)y]], (size_t)n);
+        return c ? c < 0 : length(x) != length(y) ? length(x) < length(y) : x < y;
+    });
+    // what order[from .. to) have in common from class `done` on, at most `most` classes
+    auto common = [&](size_t from, size_t to, int64_t done, int64_t most) {
+        int64_t n = std::min(most, length(order[from]) - done);
+        for (size_t i = from; i < to; ++i)
+            for (int64_t j = 0; j < n; ++j)
+                if (done + j >= length(order[i]) || code(order[i], done + j) != code(order[from], done + j)) n = j;
+        return n;
+    };
+    const size_t sets = (order.size() + 1023) / 1024;
+    g->n_groups = (int32_t)((order.size() + 31) / 32);
+    g->prefix.assign(sets * 32, make_uint2(0, 0));
+    g->rest.assign(sets * 1024, make_uint4(0, 0, ~0u, 0));
+    for (size_t s = 0; s < sets; ++s) {
+        const size_t end = std::min(order.size(), (s + 1) * 1024);
+        const int64_t m = common(s * 1024, end, 0, GRAMMAR_SHARED);
+        g->super.push_back((uint32_t)classes(order[s * 1024], 0, m, GRAMMAR_SHARED));
+        g->super_steps = std::max(g->super_steps, (int32_t)m);
+        for (size_t k = s * 32; k * 32 < end; ++k) {
+            const size_t last = std::min(end, k * 32 + 32);
+            const int64_t n = common(k * 32, last, m, GRAMMAR_SHARED);
+            int64_t steps = 1;                                // (0 says that there is no group)
+            for (size_t i = k * 32; i < last; ++i) {
+                const int32_t v = order[i];
+                steps = std::max(steps, length(v) - m - n);
+                const uint64_t rest = classes(v, m + n, length(v), GRAMMAR_REST);
+                g->rest[i] = make_uint4((uint32_t)rest, (uint32_t)(rest >> 32), (uint32_t)v, 0);
+            }
+            g->prefix[k] = make_uint2((uint32_t)classes(order[k * 32], m, m + n, GRAMMAR_SHARED), (uint32_t)(steps > GRAMMAR_REST ? GRAMMAR_SLOW : steps));
+            g->prefix_steps = std::max(g->prefix_steps, (int32_t)n);
+        }
+    }
+}
+
+// The automaton for masks (see GrammarTables).
+void make_steps(dnatok_grammar* g) {
+    const int64_t columns = 1ll << g->log_pitch;
+    g->step32.resize((size_t)((g->n_states + 1) * columns));
+    for (int64_t s = 0; s <= g->n_states; ++s)
+        for (int64_t c = 0; c < columns; ++c) {
+            const int32_t to = s == g->n_states ? -1 : c == columns - 1 ? (int32_t)s : g->next[(size_t)(s * columns + c)];
+            g->step32[(size_t)(s * columns + c)] = (uint32_t)(to < 0 ? g->n_states : to) << g->log_pitch;
+        }
+    if ((g->n_states + 1ll) * columns <= 1 << 16) {
+        g->step16.assign(g->step32.begin(), g->step32.end());
+        g->step32.clear();
+    }
 }
 
 }  // namespace
@@ -285,14 +524,21 @@ int dnatok_create_grammar(const int32_t* next, int32_t n_states, int32_t n_class
     try {
         auto* g = new dnatok_grammar();
         struct Undo { dnatok_grammar* g; ~Undo() { delete g; } } undo{g};
-        g->n_states = n_states; g->n_classes = n_classes; g->width = width; g->end_id = end_id;
-        g->next.assign(next, next + (int64_t)n_states * n_classes);
+        g->n_states = n_states; g->width = width; g->end_id = end_id;
+        while (1 << g->log_pitch < n_classes + 1) ++g->log_pitch;
+        g->next.assign((size_t)n_states << g->log_pitch, -1);
+        for (int64_t s = 0; s < n_states; ++s)
+            for (int32_t c = 0; c < n_classes; ++c) g->next[(size_t)((s << g->log_pitch) + c)] = next[s * n_classes + c];
         g->accepting.resize((size_t)n_states);
         for (int32_t i = 0; i < n_states; ++i) g->accepting[(size_t)i] = accepting[i] != 0;
         g->codes.resize((size_t)total);
         for (int64_t i = 0; i < total; ++i) g->codes[(size_t)i] = byte_class[token_bytes[i]];
         g->token_at.resize((size_t)width + 1);
         for (int64_t v = 0; v <= width; ++v) g->token_at[(size_t)v] = (int32_t)token_offsets[v];
+        if (n_classes <= 15 && n_states < 1 << 27) {
+            sort_tokens(g);
+            make_steps(g);
+        }
         undo.g = nullptr;
         *out = g;
     } catch (const std::bad_alloc&) {
@@ -323,7 +569,7 @@ int dnatok_grammar_allowed(dnatok_grammar* g, const int32_t* d_states, int64_t n
     if (n_rows == 0) return DNATOK_OK;
     GrammarTables t;
     if (int rc = grammar_tables(g, (cudaStream_t)stream, &t)) return rc;
-    return launch_allowed(t, d_states, n_rows, d_allowed, (cudaStream_t)stream);
+    return launch_allowed(t, d_states, nullptr, 0, nullptr, n_rows, d_allowed, (cudaStream_t)stream);
 }
 
 int dnatok_grammar_step(dnatok_grammar* g, const int32_t* d_states, const void* d_tokens, int32_t token_bits, int64_t n_rows,
@@ -338,9 +584,10 @@ int dnatok_grammar_step(dnatok_grammar* g, const int32_t* d_states, const void* 
     GrammarTables t;
     cudaStream_t st = (cudaStream_t)stream;
     if (int rc = grammar_tables(g, st, &t)) return rc;
+    if (d_allowed) return launch_allowed(t, d_states, d_tokens, token_bits, d_states_out, n_rows, d_allowed, st);
     grammar_advance_kernel<<<(unsigned)((n_rows + GRAMMAR_THREADS - 1) / GRAMMAR_THREADS), GRAMMAR_THREADS, 0, st>>>(t, d_states, d_tokens, token_bits, n_rows, d_states_out);
     LAUNCH_CHECK("grammar_advance_kernel");
-    return d_allowed ? launch_allowed(t, d_states_out, n_rows, d_allowed, st) : DNATOK_OK;
+    return DNATOK_OK;
 }
 
 }  // extern "C"

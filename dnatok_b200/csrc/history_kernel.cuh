@@ -43,24 +43,110 @@ __device__ __forceinline__ int64_t history_row(const HistoryArgs& a, int64_t row
     return h >= 0 && h < a.history_rows ? h : -1;
 }
 
-// A warp takes a row; its lanes take the row's ids in turn.
+// Rows shorter than the vocabulary: `group` threads (a power of two) of one of `splits` parts of a row take its ids in turn
+// and enter them where they belong.  Four ids a thread are under way at a time.
 template <typename IdT>
 __global__ void __launch_bounds__(HISTORY_THREADS)
-history_add_kernel(HistoryArgs a, const IdT* __restrict__ ids) {
-    const int lane = threadIdx.x & 31;
+history_add_kernel(HistoryArgs a, const IdT* __restrict__ ids, int group, int splits) {
     const int64_t words = (a.width + 31) / 32;
-    const int64_t warps = (int64_t)gridDim.x * (HISTORY_THREADS / 32);
-    for (int64_t row = (int64_t)blockIdx.x * (HISTORY_THREADS / 32) + (threadIdx.x >> 5); row < a.n_rows; row += warps) {
-        int64_t lo, hi;
-        const int64_t h = history_row(a, row, &lo, &hi);
-        if (h < 0) continue;
-        for (int64_t i = lo + lane; i < hi; i += 32) {
-            const int64_t id = (int64_t)ids[i];
-            if (id < 0 || id >= a.width) continue;
-            atomicOr(a.seen + h * words + (id >> 5), 1u << (id & 31));
-            if (a.counts) atomicAdd(a.counts + h * a.width + id, 1);
+    const int64_t unit = ((int64_t)blockIdx.x * HISTORY_THREADS + threadIdx.x) / group;
+    const int64_t row = unit / splits;
+    if (row >= a.n_rows) return;
+    int64_t lo, hi;
+    const int64_t h = history_row(a, row, &lo, &hi);
+    if (h < 0) return;
+    uint32_t* seen = a.seen + h * words;
+    int32_t* counts = a.counts ? a.counts + h * a.width : nullptr;
+    const int64_t step = (int64_t)group * splits;
+    for (int64_t i = lo + (unit % splits) * group + (threadIdx.x & (group - 1)); i < hi; i += 4 * step) {
+        int64_t id[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) id[k] = i + k * step < hi ? (int64_t)ids[i + k * step] : -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (id[k] < 0 || id[k] >= a.width) continue;
+            atomicOr(seen + (id[k] >> 5), 1u << (id[k] & 31));
+            if (counts) atomicAdd(counts + id[k], 1);
         }
     }
+}
+
+constexpr int HISTORY_LONG_THREADS = 512;
+
+// The part of a row that one of `splits` blocks takes.
+__device__ __forceinline__ void history_part(int64_t& lo, int64_t& hi, int split, int splits) {
+    const int64_t each = (hi - lo + splits - 1) / splits;
+    const int64_t end = hi;
+    lo += each * split;
+    hi = lo + each < end ? lo + each : end;
+}
+
+// Long rows, counted: a block counts its part of a row in shared memory and then adds what it found.  A long row of few
+// different tokens (bases) would queue up at a handful of counters: there are 2^log_copies of each, one for every 32 / copies
+// lanes of a warp, in banks of their own.
+template <typename IdT>
+__global__ void __launch_bounds__(HISTORY_LONG_THREADS)
+history_count_kernel(HistoryArgs a, const IdT* __restrict__ ids, int splits, int log_copies) {
+    extern __shared__ int32_t found[];            // [width][copies]
+    const int64_t row = blockIdx.x / splits;
+    int64_t lo, hi;
+    const int64_t h = history_row(a, row, &lo, &hi);
+    if (h < 0) return;
+    history_part(lo, hi, (int)(blockIdx.x % splits), splits);
+    if (lo >= hi) return;
+    const int width = (int)a.width, copies = 1 << log_copies;
+    for (int v = threadIdx.x; v < width << log_copies; v += HISTORY_LONG_THREADS) found[v] = 0;
+    __syncthreads();
+    const int copy = threadIdx.x & (copies - 1);
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 8 * HISTORY_LONG_THREADS) {
+        int64_t id[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) id[k] = i + k * HISTORY_LONG_THREADS < hi ? (int64_t)ids[i + k * HISTORY_LONG_THREADS] : -1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (id[k] >= 0 && id[k] < width) atomicAdd(found + (((int)id[k] << log_copies) | copy), 1);
+    }
+    __syncthreads();
+    const int words = (width + 31) / 32;
+    for (int v = threadIdx.x; v < words * 32; v += HISTORY_LONG_THREADS) {
+        int32_t n = 0;
+        if (v < width)
+            for (int k = 0; k < copies; ++k) n += found[(v << log_copies) | ((v + k) & (copies - 1))];   // (lanes start at banks of their own)
+        const uint32_t word = __ballot_sync(0xffffffffu, n > 0);
+        if (n > 0) atomicAdd(a.counts + h * a.width + v, n);
+        if (word && (threadIdx.x & 31) == 0) atomicOr(a.seen + h * words + (v >> 5), word);
+    }
+}
+
+// Long rows, only marked: the same with a bit per token; a bit that is there already is not set again.
+template <typename IdT>
+__global__ void __launch_bounds__(HISTORY_LONG_THREADS)
+history_mark_kernel(HistoryArgs a, const IdT* __restrict__ ids, int splits) {
+    extern __shared__ uint32_t marked[];          // [words]
+    const int64_t row = blockIdx.x / splits;
+    int64_t lo, hi;
+    const int64_t h = history_row(a, row, &lo, &hi);
+    if (h < 0) return;
+    history_part(lo, hi, (int)(blockIdx.x % splits), splits);
+    if (lo >= hi) return;
+    const int width = (int)a.width, words = (width + 31) / 32;
+    for (int w = threadIdx.x; w < words; w += HISTORY_LONG_THREADS) marked[w] = 0;
+    __syncthreads();
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 8 * HISTORY_LONG_THREADS) {
+        int64_t id[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) id[k] = i + k * HISTORY_LONG_THREADS < hi ? (int64_t)ids[i + k * HISTORY_LONG_THREADS] : -1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (id[k] < 0 || id[k] >= width) continue;
+            uint32_t* word = marked + ((int)id[k] >> 5);
+            const uint32_t bit = 1u << (id[k] & 31);
+            if (!(*reinterpret_cast<volatile uint32_t*>(word) & bit)) atomicOr(word, bit);
+        }
+    }
+    __syncthreads();
+    for (int w = threadIdx.x; w < words; w += HISTORY_LONG_THREADS)
+        if (marked[w]) atomicOr(a.seen + h * words + w, marked[w]);
 }
 
 }  // namespace dnatok

@@ -325,8 +325,8 @@ def _penalty(a, name: str, v, n: int, device, keep: list) -> bool:
         keep.append(v)
         return True
     v = float(v)
-    if name == "repetition" and not 0 < v < float("inf"):
-        raise ValueError("repetition must be positive and finite")
+    if name == "repetition" and not 2.0 ** -126 <= v <= 2.0 ** 126:
+        raise ValueError("repetition must be positive and finite (2^-126 to 2^126)")
     if v != v or v in (float("inf"), -float("inf")):
         raise ValueError("%s must be finite" % name)
     setattr(a, name, v)
@@ -471,7 +471,7 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
     bias and mask, as a new tensor of its type or of ``out_dtype`` float32, or in ``out`` (which may be ``logits``).
 
     * A token the row has seen: ``x > 0 ? x / repetition : x * repetition``; one it generated ``c > 0`` times, then
-      ``- frequency * c - presence``.  Each is a number, or a float32 tensor [n] (repetition positive there too).
+      ``- frequency * c - presence``.  Each is a number, or a float32 tensor [n] (repetition from 2^-126 to 2^126 there too).
       ``rows`` [n] names each row's history row (a row outside the history has none); two rows may share one.
     * ``bias`` float32 [width] or [n, width] is added.
     * ``allowed`` int32 [n, words] or [words]: tokens whose bit is 0 become ``-inf`` whatever their logits hold, NaN

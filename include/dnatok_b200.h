@@ -310,7 +310,8 @@ typedef struct {
 } dnatok_logits;
 
 /* out = allowed ? x2 + bias : -inf, where a token that the row has seen has x1 = x > 0 ? x / repetition : x * repetition
- * and one that it generated c > 0 times x2 = x1 - frequency * c - presence; other tokens keep x.  Computed in 32 bits,
+ * (repetition from 2^-126 to 2^126) and one that it generated c > 0 times x2 = x1 - frequency * c - presence; other tokens
+ * keep x.  Computed in 32 bits,
  * rounded once to the output's type: that of the logits or DNATOK_F32.  Logits that are not allowed have no influence, NaN
  * included; a row without an allowed token is -inf throughout.  d_out may be the logits themselves (same type and stride);
  * another overlap is not allowed. */
