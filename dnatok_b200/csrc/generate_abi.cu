@@ -53,10 +53,13 @@ int check_rows(const void* rows, int bits, int64_t n_rows, int64_t history_rows)
     return 0;
 }
 
+constexpr int64_t LOGITS_MOST = INT32_MAX - 1024 * 1024;        // rows or columns: what is added to them stays in 32 bits
+
 int check_logits(const dnatok_logits* in) {
     if (!in) return abi_fail(DNATOK_ERR_INVALID, "NULL argument");
     if (!known(in->dtype)) return abi_fail(DNATOK_ERR_INVALID, "unknown type of logits");
-    if (in->n_rows < 0 || in->width < 1 || in->width > INT32_MAX) return abi_fail(DNATOK_ERR_INVALID, "bad number of rows or columns");
+    if (in->n_rows < 0 || in->n_rows > LOGITS_MOST || in->width < 1 || in->width > LOGITS_MOST)
+        return abi_fail(DNATOK_ERR_INVALID, "bad number of rows or columns");
     if (in->stride < 0) return abi_fail(DNATOK_ERR_INVALID, "stride < 0");
     if (in->n_rows && !in->logits) return abi_fail(DNATOK_ERR_INVALID, "logits is NULL");
     if (!aligned(in->logits, size_of(in->dtype))) return abi_fail(DNATOK_ERR_INVALID, "misaligned logits");
@@ -77,7 +80,7 @@ int check_logits(const dnatok_logits* in) {
 
 LogitsArgs logits_args(const dnatok_logits* in) {
     LogitsArgs a;
-    a.n_rows = in->n_rows; a.width = in->width; a.stride = in->stride;
+    a.n_rows = (int32_t)in->n_rows; a.width = (int32_t)in->width; a.stride = in->stride;
     a.seen = in->seen; a.counts = in->counts; a.history_rows = (int32_t)in->history_rows;
     a.rows = in->rows; a.rows_bits = in->rows_bits;
     a.repetition = in->repetition; a.frequency = in->frequency; a.presence = in->presence;
@@ -104,24 +107,36 @@ int64_t rows_per_block(int64_t n_rows, int64_t groups) {
     return per_warp * LOGITS_WARPS;
 }
 
-// A block for every tile of columns and group of rows.  Each warp gets one row where there are few blocks, then as many
-// rows as leave about 16 blocks an SM: their loads of what belongs to the columns, and the partial sums of a bias' gradient,
-// are spread over those rows.
-dim3 logits_grid(int64_t n_rows, int64_t width) {
-    const int64_t tiles = (width + LOGITS_TILE - 1) / LOGITS_TILE;
-    int64_t groups = ((int64_t)SMS * 16 + tiles - 1) / tiles;
+int64_t tiles_of(int64_t width, int parts) { return (width + LOGITS_PART * parts - 1) / (LOGITS_PART * parts); }
+
+// Parts a tile (see logits_kernel.cuh): one as long as that gives at most 4 warps to each of the GPU's schedulers.
+int logits_parts(int64_t n_rows, int64_t width) { return n_rows * tiles_of(width, 1) <= (int64_t)SMS * 16 ? 1 : 2; }
+
+// A warp for every tile of columns and row.
+dim3 logits_grid(int64_t n_rows, int64_t width, int parts) {
+    const int64_t groups = (n_rows + LOGITS_WARPS - 1) / LOGITS_WARPS;
+    return dim3((unsigned)tiles_of(width, parts), (unsigned)(groups < 65535 ? groups : 65535));
+}
+
+// With a shared bias' gradient a block goes through several groups of rows, as many as leave about 8 blocks an SM: their
+// partial sums are few beside what they read.
+dim3 bias_grid(int64_t n_rows, int64_t width, int parts) {
+    const int64_t tiles = tiles_of(width, parts);
+    int64_t groups = ((int64_t)SMS * 8 + tiles - 1) / tiles;
     const int64_t most = (n_rows + LOGITS_WARPS - 1) / LOGITS_WARPS;
     if (groups > most) groups = most;
     const int64_t rows = rows_per_block(n_rows, groups);
     return dim3((unsigned)tiles, (unsigned)((n_rows + rows - 1) / rows));
 }
 
-// Which columns a lane takes (see logits_kernel.cuh).
+// Which columns a lane takes, whether there is a history, and the parts of a tile (see logits_kernel.cuh).
 template <size_t S, size_t U, typename F>
-void with_map(bool vector, int64_t width, F f) {
+void with_variant(bool vector, int64_t width, bool seen, int parts, F f) {
     constexpr int MAP = (S > 2 || U > 2) ? HALVES : CONTIGUOUS;
-    if (!vector || width % (MAP == HALVES ? 4 : 8)) f(std::integral_constant<int, APART>());
-    else f(std::integral_constant<int, MAP>());
+    auto tiled = [&](auto m, auto s) { if (parts == 1) f(m, s, std::integral_constant<int, 1>()); else f(m, s, std::integral_constant<int, 2>()); };
+    auto known = [&](auto m) { if (seen) tiled(m, std::true_type()); else tiled(m, std::false_type()); };
+    if (!vector || width % (MAP == HALVES ? 4 : 8)) known(std::integral_constant<int, APART>());
+    else known(std::integral_constant<int, MAP>());
 }
 
 // Calls f with a null pointer of the element type.
@@ -148,14 +163,22 @@ int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtyp
     const bool vector = vector_rows(in->logits, in->stride, size_of(in->dtype), in->n_rows) &&
                         vector_rows(d_out, out_stride, size_of(out_dtype), in->n_rows) &&
                         vector_rows(in->bias, in->bias_stride, 4, in->n_rows);
-    const int64_t groups = (a.n_rows + LOGITS_WARPS - 1) / LOGITS_WARPS;
-    const dim3 grid((unsigned)((a.width + LOGITS_TILE - 1) / LOGITS_TILE), (unsigned)(groups < 65535 ? groups : 65535));
+    const int parts = logits_parts(a.n_rows, a.width);
+    const dim3 grid = logits_grid(a.n_rows, a.width, parts);
+    const int64_t logits = (int64_t)a.n_rows * a.width;
+    const bool few = logits <= (int64_t)SMS * 2048;                   // a thread each, all of them on the GPU at once
     with_type(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         auto typed = [&](auto* o) {
             using O = std::remove_pointer_t<decltype(o)>;
-            with_map<sizeof(T), sizeof(O)>(vector, a.width, [&](auto m) {
-                process_logits_kernel<T, O, decltype(m)::value><<<grid, LOGITS_THREADS, 0, st>>>(a, (const T*)in->logits, (O*)d_out, out_stride);
+            if (few) {
+                process_each_kernel<T, O><<<(unsigned)((logits + LOGITS_THREADS - 1) / LOGITS_THREADS), LOGITS_THREADS, 0, st>>>(
+                    a, (const T*)in->logits, (O*)d_out, out_stride);
+                return;
+            }
+            with_variant<sizeof(T), sizeof(O)>(vector, a.width, a.seen != nullptr, parts, [&](auto m, auto seen, auto n) {
+                process_logits_kernel<T, O, decltype(m)::value, decltype(seen)::value, decltype(n)::value><<<grid, LOGITS_THREADS, 0, st>>>(
+                    a, (const T*)in->logits, (O*)d_out, out_stride);
             });
         };
         if (out_dtype == in->dtype) typed(t); else typed((float*)nullptr);
@@ -166,7 +189,7 @@ int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtyp
 
 size_t dnatok_logits_scratch_bytes(int64_t n_rows, int64_t width) {
     if (n_rows < 1 || width < 1) return 0;
-    const unsigned blocks = logits_grid(n_rows, width).y;
+    const unsigned blocks = bias_grid(n_rows, width, logits_parts(n_rows, width)).y;
     return blocks > 1 ? (size_t)blocks * (size_t)width * 4 : 0;
 }
 
@@ -193,9 +216,10 @@ int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, 
                         vector_rows(d_grad, grad_stride, size_of(grad_dtype), in->n_rows) &&
                         vector_rows(d_dlogits, dlogits_stride, size_of(in->dtype), in->n_rows) &&
                         (shared || vector_rows(d_dbias, in->width, 4, in->n_rows));
-    const dim3 grid = logits_grid(a.n_rows, a.width);
-    const int rows = (int)rows_per_block(a.n_rows, grid.y);
-    const bool join = d_dbias && shared && grid.y > 1;
+    const bool add = d_dbias && shared;
+    const int parts = logits_parts(a.n_rows, a.width);
+    const dim3 grid = add ? bias_grid(a.n_rows, a.width, parts) : logits_grid(a.n_rows, a.width, parts);
+    const bool join = add && grid.y > 1;
     if (join && (!d_scratch || scratch_bytes < dnatok_logits_scratch_bytes(a.n_rows, a.width) || !aligned(d_scratch, 256)))
         return abi_fail(DNATOK_ERR_SCRATCH, "the gradient of a shared bias needs %zu bytes of 256-byte aligned scratch",
                         dnatok_logits_scratch_bytes(a.n_rows, a.width));
@@ -204,14 +228,16 @@ int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, 
         using T = std::remove_pointer_t<decltype(t)>;
         auto typed = [&](auto* g) {
             using G = std::remove_pointer_t<decltype(g)>;
-            with_map<sizeof(T), sizeof(G)>(vector, a.width, [&](auto m) {
-                constexpr int MAP = decltype(m)::value;
-                if (d_dbias && shared)
-                    logits_gradient_kernel<T, G, MAP, true><<<grid, LOGITS_THREADS, 0, st>>>(
-                        a, (const T*)in->logits, (const G*)d_grad, grad_stride, (T*)d_dlogits, dlogits_stride, sums, rows);
+            with_variant<sizeof(T), sizeof(G)>(vector, a.width, a.seen && d_dlogits, parts, [&](auto m, auto seen, auto n) {
+                constexpr int MAP = decltype(m)::value, PARTS = decltype(n)::value;
+                constexpr bool SEEN = decltype(seen)::value;
+                if (add)
+                    logits_bias_gradient_kernel<T, G, MAP, SEEN, PARTS><<<grid, LOGITS_THREADS, 0, st>>>(
+                        a, (const T*)in->logits, (const G*)d_grad, grad_stride, (T*)d_dlogits, dlogits_stride, sums,
+                        (int)rows_per_block(a.n_rows, grid.y));
                 else
-                    logits_gradient_kernel<T, G, MAP, false><<<grid, LOGITS_THREADS, 0, st>>>(
-                        a, (const T*)in->logits, (const G*)d_grad, grad_stride, (T*)d_dlogits, dlogits_stride, d_dbias, rows);
+                    logits_gradient_kernel<T, G, MAP, SEEN, PARTS><<<grid, LOGITS_THREADS, 0, st>>>(
+                        a, (const T*)in->logits, (const G*)d_grad, grad_stride, (T*)d_dlogits, dlogits_stride, d_dbias);
             });
         };
         if (grad_dtype == in->dtype) typed(t); else typed((float*)nullptr);

@@ -10,6 +10,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "common.cuh"
 
 namespace dnatok {
@@ -17,7 +18,8 @@ namespace dnatok {
 constexpr int LOGITS_THREADS = 256;
 
 struct LogitsArgs {
-    int64_t n_rows, width, stride;
+    int32_t n_rows, width;
+    int64_t stride;
     const uint32_t* seen;         // [history_rows, words] or NULL
     const int32_t* counts;        // [history_rows, width] or NULL: no row generated anything
     int32_t history_rows;
@@ -40,21 +42,47 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // The history row of a row, -1 for none.
-__device__ __forceinline__ int32_t history_of(const LogitsArgs& a, int64_t row) {
-    if (!a.rows) return (int32_t)row;
+__device__ __forceinline__ int32_t history_of(const LogitsArgs& a, int32_t row) {
+    if (!a.rows) return row;
     const int64_t h = a.rows_bits == 64 ? __ldg(static_cast<const int64_t*>(a.rows) + row) : __ldg(static_cast<const int32_t*>(a.rows) + row);
     return h >= 0 && h < a.history_rows ? (int32_t)h : -1;
 }
-__device__ __forceinline__ float of_row(const float* each, float all, int64_t row) { return each ? __ldg(each + row) : all; }
+__device__ __forceinline__ float of_row(const float* each, float all, int32_t row) { return each ? __ldg(each + row) : all; }
 
-// A block keeps one tile of 512 columns and goes through rows of it, a warp a row, 8 columns a lane in each of the tile's
-// two parts: what belongs to the columns is worked out once, neighbouring blocks read neighbouring columns of the same
-// rows, and a row's own words and numbers are fetched for 16 columns a lane.
-// Which columns of a part a lane has (MAP):
+__device__ __forceinline__ bool bit_at(const uint32_t* words, int v) { return __ldg(words + (v >> 5)) >> (v & 31) & 1; }
+
+// Small calls, a thread a logit: nothing is shared, but few instructions stand between the loads (64 rows of 4,106 bf16
+// logits with everything: 4.2 us, the kernel below 6.2).
+template <typename T, typename O>
+__global__ void __launch_bounds__(LOGITS_THREADS)
+process_each_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
+    const uint32_t i = blockIdx.x * LOGITS_THREADS + threadIdx.x;
+    if (i >= (uint32_t)a.n_rows * (uint32_t)a.width) return;
+    const int row = (int)(i / (uint32_t)a.width), v = (int)(i - (uint32_t)row * (uint32_t)a.width);
+    float y = as_float(logits[row * a.stride + v]);
+    const bool ok = !a.allowed || bit_at(a.allowed + row * a.allowed_stride, v);
+    const int32_t h = a.seen ? history_of(a, row) : -1;
+    if (h >= 0 && bit_at(a.seen + (int64_t)h * ((a.width + 31) >> 5), v)) {
+        const int32_t c = a.counts ? __ldg(a.counts + ((int64_t)h * a.width + v)) : 0;
+        const float r = of_row(a.d_repetition, a.repetition, row);
+        y *= y > 0.f ? __frcp_rn(r) : r;
+        if (c > 0) y = y - of_row(a.d_frequency, a.frequency, row) * (float)c - of_row(a.d_presence, a.presence, row);
+    }
+    if (a.bias) y += __ldg(a.bias + row * a.bias_stride + v);
+    out[row * out_stride + v] = from_float<O>(ok ? y : -INFINITY);
+}
+
+// A warp takes a tile of one or two parts (PARTS) of 256 columns of a row, 8 columns a lane in each: two where that leaves
+// warps for the whole GPU, since a row's own words and numbers are then fetched for twice as many columns.  Which columns of
+// a part a lane has (MAP):
 //   CONTIGUOUS  8 neighbouring ones, for 16-bit arrays that begin and go on at multiples of 16 bytes: one access each
 //   HALVES      4 and 4 at a distance of 128, where a 32-bit array is among them: its two accesses fill whole sectors
 //   APART       32 apart, at any alignment (a vocabulary of 4,106 tokens in 16 bits, a view that begins anywhere)
-constexpr int LOGITS_PART = 256, LOGITS_PARTS = 2, LOGITS_TILE = LOGITS_PART * LOGITS_PARTS;
+//
+// All columns get bias and mask on this way.  The tokens that a row has seen are few among many, as a rule; penalising 8
+// columns a lane for one of them took more instructions than all the rest together.  So the hits (seen and allowed) are
+// mended afterwards: the warp lists their columns in shared memory and takes 32 of them at a time.
+constexpr int LOGITS_PART = 256;
 constexpr int LOGITS_WARPS = LOGITS_THREADS / 32;
 constexpr int LOGITS_BLOCKS = 4;                   // an SM: 64 registers a thread
 enum { APART, CONTIGUOUS, HALVES };
@@ -62,9 +90,6 @@ enum { APART, CONTIGUOUS, HALVES };
 template <int MAP> __device__ __forceinline__ int tile_column(int lane, int j) {
     return MAP == CONTIGUOUS ? lane * 8 + j : MAP == HALVES ? (j >> 2) * 128 + lane * 4 + (j & 3) : j * 32 + lane;
 }
-
-// Columns of the row from this block's tile on, at most a tile's.
-__device__ __forceinline__ int tile_left(int64_t width, int64_t base) { return width - base < LOGITS_TILE ? (int)(width - base) : LOGITS_TILE; }
 
 // Bit j: column j of this lane lies in the row, of which `left` columns are left from the part on.  (Widths of the maps with
 // neighbouring columns are multiples of what a lane moves at a time: those columns lie in the row together or not at all.)
@@ -77,9 +102,10 @@ template <int MAP> __device__ __forceinline__ uint32_t tile_all(int left, int la
     return b;
 }
 
-// A set's words of this tile, lane l holding word l % 16; and bit j: the set holds column j of this lane in part u.
-__device__ __forceinline__ uint32_t tile_word(const uint32_t* words, int left, int lane) {
-    return (lane & 15) * 32 < left ? __ldg(words + (lane & 15)) : 0;
+// A set's words of this tile, lane l holding word l % (8 PARTS); and bit j: the set holds column j of this lane in part u.
+template <int PARTS> __device__ __forceinline__ uint32_t tile_word(const uint32_t* words, int left, int lane) {
+    const int w = lane & (8 * PARTS - 1);
+    return w * 32 < left ? __ldg(words + w) : 0;
 }
 template <int MAP> __device__ __forceinline__ uint32_t tile_bits(uint32_t word, int u, int lane) {
     constexpr uint32_t FULL = 0xffffffffu;
@@ -117,12 +143,39 @@ __device__ __forceinline__ void load_tile(const T* p, uint32_t want, int lane, R
     }
 }
 
+// The values rounded, two an instruction where the type has one, and -inf where `may` has no bit.
+__device__ __forceinline__ void round_all(const float (&y)[8], uint32_t may, Raw8<float>& raw) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) raw.v[j] = may >> j & 1 ? y[j] : -INFINITY;
+}
+__device__ __forceinline__ uint32_t round_two(float x, float y, __half) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t round_two(float x, float y, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T> __device__ __forceinline__ void round_all(const float (&y)[8], uint32_t may, Raw8<T>& raw) {
+    constexpr uint32_t NONE = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;     // -inf twice
+    uint32_t* words = reinterpret_cast<uint32_t*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        // bit j of four into the top bit of byte j; a byte's top bit then fills the 16 bits of a value
+        const uint32_t tops = (may >> 4 * i & 0xf) * 0x10204080u;
+        uint32_t m0, m1;
+        asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m0) : "r"(tops));
+        asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m1) : "r"(tops));
+        words[2 * i] = (round_two(y[4 * i], y[4 * i + 1], T()) & m0) | (NONE & ~m0);
+        words[2 * i + 1] = (round_two(y[4 * i + 2], y[4 * i + 3], T()) & m1) | (NONE & ~m1);
+    }
+}
+
 template <int MAP, typename T>
-__device__ __forceinline__ void store_tile(T* p, uint32_t all, int lane, const float (&y)[8]) {
+__device__ __forceinline__ void store_tile(T* p, uint32_t all, int lane, const float (&y)[8], uint32_t may = 0xff) {
     constexpr int EACH = MAP == APART ? 1 : MAP == HALVES ? 4 : 8;
     Raw8<T> raw;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) raw.v[j] = from_float<T>(y[j]);
+    round_all(y, may, raw);
 #pragma unroll
     for (int k = 0; k < 8 / EACH; ++k) {
         if (!(all >> k * EACH & 1)) continue;
@@ -143,190 +196,229 @@ __device__ __forceinline__ void store_tile(T* p, uint32_t all, int lane, const f
 // x / r of a seen token is x * (1 / r): two roundings in 32 bits instead of one, and no division a token.
 struct Penalty { float up, down; };
 __device__ __forceinline__ Penalty penalty_of(float r) { return {__frcp_rn(r), r}; }
+__device__ __forceinline__ float penalise(const Penalty& q, float x, float by) { return by * (x > 0.f ? q.up : q.down); }
 
-// *p where `want` is not 0, else 0: one predicated load, not a branch.
-__device__ __forceinline__ int32_t load_where(const int32_t* p, uint32_t want) {
-    int32_t v = 0;
-    asm("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q ld.global.nc.s32 %0, [%1];\n}" : "+r"(v) : "l"(p), "r"(want));
-    return v;
+// The hits of the tile that this lane lists, from the tile's words: bit j stands for column hit_column(lane) + j.
+template <int PARTS> __device__ __forceinline__ int hit_shift(int lane) { return lane / (8 * PARTS) * (8 * PARTS); }
+template <int PARTS> __device__ __forceinline__ int hit_column(int lane) { return (lane & (8 * PARTS - 1)) * 32 + hit_shift<PARTS>(lane); }
+
+template <int PARTS>
+__device__ __forceinline__ uint32_t tile_hits(const LogitsArgs& a, int32_t h, uint32_t ok, int base, int left, int lane) {
+    if (h < 0) return 0;
+    constexpr int BITS = 8 * PARTS;
+    const uint32_t word = tile_word<PARTS>(a.seen + ((int64_t)h * ((a.width + 31) >> 5) + (base >> 5)), left, lane) & ok;
+    const int behind = left - hit_column<PARTS>(lane);        // (bits behind the last column are no tokens)
+    return word >> hit_shift<PARTS>(lane) & ((1u << (behind >= BITS ? BITS : behind > 0 ? behind : 0)) - 1);
 }
 
-template <typename T, typename O, int MAP>
-__global__ void __launch_bounds__(LOGITS_THREADS, LOGITS_BLOCKS)
-process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
-    const int lane = threadIdx.x & 31;
-    const int64_t base = (int64_t)blockIdx.x * LOGITS_TILE;
-    const int left = tile_left(a.width, base);
-    const int words = ((int)a.width + 31) >> 5;
-#pragma unroll 1
-    for (int64_t row = (int64_t)blockIdx.y * LOGITS_WARPS + (threadIdx.x >> 5); row < a.n_rows; row += (int64_t)gridDim.y * LOGITS_WARPS) {
-        const T* x_row = logits + row * a.stride + base;
-        Raw8<T> x[LOGITS_PARTS];
+// The columns of a warp's hits, in their order, into `list`; how many there are.
+template <int PARTS>
+__device__ __forceinline__ int list_hits(uint32_t hits, uint16_t* list, int lane) {
+    const int mine = __popc(hits);
+    int upto = mine;                                          // hits of the lanes up to this one
 #pragma unroll
-        for (int u = 0; u < LOGITS_PARTS; ++u) {
+    for (int d = 1; d < 32; d *= 2) {
+        const int before = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += before;
+    }
+    uint16_t* to = list + (upto - mine);
+    for (; hits; hits &= hits - 1) *to++ = (uint16_t)(hit_column<PARTS>(lane) + __ffs(hits) - 1);
+    __syncwarp();
+    return __shfl_sync(0xffffffffu, upto, 31);
+}
+
+// A tile's values as they were before this warp wrote over them, by column.
+template <int MAP, typename T>
+__device__ __forceinline__ void keep_tile(T* kept, const Raw8<T>& raw, int lane) {
+    constexpr int EACH = MAP == APART ? 1 : MAP == HALVES ? 4 : 8;
+#pragma unroll
+    for (int k = 0; k < 8 / EACH; ++k) {
+        T* q = kept + tile_column<MAP>(lane, k * EACH);
+        const T* from = raw.v + k * EACH;
+        if constexpr (EACH == 1) {
+            *q = *from;
+        } else if constexpr (EACH * sizeof(T) == 8) {
+            *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(from);
+        } else {
+#pragma unroll
+            for (int i = 0; i < (int)(EACH * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(q)[i] = reinterpret_cast<const uint4*>(from)[i];
+        }
+    }
+}
+
+template <typename T, typename O, int MAP, bool SEEN, int PARTS>
+__global__ void __launch_bounds__(LOGITS_THREADS, 6)
+process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
+    __shared__ Raw8<T> kept[SEEN ? LOGITS_WARPS : 1][LOGITS_PART * PARTS / 8];
+    __shared__ uint16_t listed[SEEN ? LOGITS_WARPS : 1][LOGITS_PART * PARTS];
+    const int lane = threadIdx.x & 31;
+    const int base = blockIdx.x * LOGITS_PART * PARTS, left = a.width - base;
+#pragma unroll 1
+    for (int row = blockIdx.y * LOGITS_WARPS + (threadIdx.x >> 5); row < a.n_rows; row += gridDim.y * LOGITS_WARPS) {
+        const T* x_row = logits + (row * a.stride + base);
+        Raw8<T> x[PARTS];
+#pragma unroll
+        for (int u = 0; u < PARTS; ++u) {
             x[u] = {};
             load_tile<MAP>(x_row + u * LOGITS_PART, tile_all<MAP>(left - u * LOGITS_PART, lane), lane, x[u]);
         }
-        const uint32_t ok_word = a.allowed ? tile_word(a.allowed + row * a.allowed_stride + (base >> 5), left, lane) : 0xffffffffu;
-        const int32_t h = a.seen ? history_of(a, row) : -1;
-        const uint32_t hit_word = h >= 0 ? tile_word(a.seen + ((int64_t)h * words + (base >> 5)), left, lane) & ok_word : 0;
-        const bool any_hit = __any_sync(0xffffffffu, hit_word);
-        const float* b_row = a.bias ? a.bias + row * a.bias_stride + base : nullptr;
-        O* y_row = out + row * out_stride + base;
+        const uint32_t ok = a.allowed ? tile_word<PARTS>(a.allowed + (row * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
+        uint32_t hits = 0;
+        const int32_t* counts = nullptr;
+        if (SEEN) {
+            const int32_t h = history_of(a, row);
+            hits = tile_hits<PARTS>(a, h, ok, base, left, lane);
+            if (a.counts && h >= 0) counts = a.counts + ((int64_t)h * a.width + base);
+        }
+        const bool mend = SEEN && __any_sync(0xffffffffu, hits);
+        T* before = kept[SEEN ? threadIdx.x >> 5 : 0][0].v;
+        uint16_t* list = listed[SEEN ? threadIdx.x >> 5 : 0];
+        int n_hits = 0, c = 0;                                // c: of this lane's first hit, ahead of time
+        if (mend) {
+            n_hits = list_hits<PARTS>(hits, list, lane);
+            if (counts && lane < n_hits) c = __ldg(counts + list[lane]);
+        }
+        const float* bias = a.bias ? a.bias + (row * a.bias_stride + base) : nullptr;
+        O* y_row = out + (row * out_stride + base);
 #pragma unroll
-        for (int u = 0; u < LOGITS_PARTS; ++u) {
+        for (int u = 0; u < PARTS; ++u) {
             const uint32_t all = tile_all<MAP>(left - u * LOGITS_PART, lane);
+            if (mend) keep_tile<MAP>(before + u * LOGITS_PART, x[u], lane);
             float y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = as_float(x[u].v[j]);
-            if (any_hit) {
-                const uint32_t hit = tile_bits<MAP>(hit_word, u, lane) & all;
-                const Penalty pen = penalty_of(of_row(a.d_repetition, a.repetition, row));
-                if (hit) {
-                    int32_t c[8] = {};
-                    if (a.counts) {
-                        const int32_t* counts = a.counts + ((int64_t)h * (int32_t)a.width + base) + u * LOGITS_PART;
+            if (bias) {
+                Raw8<float> b;
+                load_tile<MAP>(bias + u * LOGITS_PART, all, lane, b);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) c[j] = load_where(counts + tile_column<MAP>(lane, j), hit >> j & 1);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float z = y[j] * (y[j] > 0.f ? pen.up : pen.down);
-                        y[j] = hit >> j & 1 ? z : y[j];
-                    }
-                    if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
-                        const float f = of_row(a.d_frequency, a.frequency, row), p = of_row(a.d_presence, a.presence, row);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float z = y[j] - f * (float)c[j] - p;
-                            y[j] = c[j] > 0 ? z : y[j];
-                        }
-                    }
-                }
+                for (int j = 0; j < 8; ++j) y[j] += b.v[j];
             }
-            if (b_row) {
-                Raw8<float> bias;
-                load_tile<MAP>(b_row + u * LOGITS_PART, all, lane, bias);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] += bias.v[j];
-            }
-            if (a.allowed) {
-                const uint32_t ok = tile_bits<MAP>(ok_word, u, lane);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = ok >> j & 1 ? y[j] : -INFINITY;
-            }
-            store_tile<MAP>(y_row + u * LOGITS_PART, all, lane, y);
+            store_tile<MAP>(y_row + u * LOGITS_PART, all, lane, y, a.allowed ? tile_bits<MAP>(ok, u, lane) : 0xff);
         }
+        if (!mend) continue;
+        __syncwarp();                                         // the values kept, and the order of the stores
+        const Penalty pen = penalty_of(of_row(a.d_repetition, a.repetition, row));
+        const float f = of_row(a.d_frequency, a.frequency, row), p = of_row(a.d_presence, a.presence, row);
+        for (int i = lane; i < n_hits; i += 32) {
+            const int v = list[i], now = c;
+            if (counts && i + 32 < n_hits) c = __ldg(counts + list[i + 32]);
+            const float x1 = as_float(before[v]);
+            float y = penalise(pen, x1, x1);
+            if (now > 0) y = y - f * (float)now - p;
+            if (bias) y += __ldg(bias + v);
+            y_row[v] = from_float<O>(y);
+        }
+        __syncwarp();
     }
 }
 
-// A row's logits are read only where its mask allows, its counts only where its history has a bit: a warp fetches those
-// words a row ahead, and the number of the history row two ahead, so that a row costs one trip to memory and not three.
-struct Ahead {
-    const uint32_t* allowed;      // this tile's words of the mask of the next row
-    const uint32_t* seen;         // this tile's words of history row 0; NULL: no history
-    int32_t h;                    // history row of the next row
-    uint32_t ok, hit;             // words fetched
-
-    // The words of `row`, whose history row is h; then the history row of the one after, if there is one.
-    __device__ __forceinline__ void fetch(const LogitsArgs& a, int64_t row, bool more, int left, int lane) {
-        ok = 0xffffffffu;
-        hit = 0;
-        if (allowed) {
-            ok = tile_word(allowed, left, lane);
-            allowed += a.allowed_stride * LOGITS_WARPS;
-        }
-        if (seen) {
-            if (h >= 0) hit = tile_word(seen + (int64_t)h * (((int32_t)a.width + 31) >> 5), left, lane);
-            if (more) h = history_of(a, row + LOGITS_WARPS);
-        }
+// The gradients of the logits at a row's hits, over those of its other allowed tokens.
+template <int PARTS, typename T, typename G>
+__device__ __forceinline__ void mend_gradient(const LogitsArgs& a, int row, uint32_t hits, uint16_t* list, const T* x_row, const G* g_row, T* d_row, int lane) {
+    if (!__any_sync(0xffffffffu, hits)) return;
+    const int n_hits = list_hits<PARTS>(hits, list, lane);           // (its barrier also puts the stores in order)
+    const Penalty pen = penalty_of(of_row(a.d_repetition, a.repetition, row));
+    for (int i = lane; i < n_hits; i += 32) {
+        const int v = list[i];
+        d_row[v] = from_float<T>(penalise(pen, as_float(x_row[v]), as_float(g_row[v])));
     }
-};
+    __syncwarp();
+}
 
-// The gradients of the logits and, SHARED, of a bias that all rows share: each warp adds up its rows of the block's columns
-// in registers, the warps' sums are joined in shared memory, those of several blocks by bias_gradient_kernel.  The incoming
-// gradient is read once for both, and the order of the additions depends on the sizes alone.
-template <typename T, typename G, int MAP, bool SHARED>
-__global__ void __launch_bounds__(LOGITS_THREADS, LOGITS_BLOCKS)
-logits_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_t grad_stride, T* dlogits, int64_t dlogits_stride,
-                       float* dbias, int rows_per_block) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t base = (int64_t)blockIdx.x * LOGITS_TILE;
-    const int left = tile_left(a.width, base);
-    uint32_t all[LOGITS_PARTS];
-#pragma unroll
-    for (int u = 0; u < LOGITS_PARTS; ++u) all[u] = tile_all<MAP>(left - u * LOGITS_PART, lane);
-    float acc[LOGITS_PARTS][8] = {};
-    int64_t row = (int64_t)blockIdx.y * rows_per_block + warp;
-    int rows = (int)((a.n_rows - row < rows_per_block - warp ? a.n_rows - row : rows_per_block - warp) + LOGITS_WARPS - 1) / LOGITS_WARPS;
-    const T* x_row = logits + row * a.stride + base;
-    const G* g_row = grad + row * grad_stride + base;
-    T* d_row = dlogits ? dlogits + row * dlogits_stride + base : nullptr;
-    Ahead next;
-    next.allowed = a.allowed ? a.allowed + row * a.allowed_stride + (base >> 5) : nullptr;
-    next.seen = a.seen && dlogits ? a.seen + (base >> 5) : nullptr;
-    next.h = -1;
-    if (rows > 0) {
-        if (next.seen) next.h = history_of(a, row);
-        next.fetch(a, row, rows > 1, left, lane);
-    }
+// The gradients of the logits and of a bias of every row.
+template <typename T, typename G, int MAP, bool SEEN, int PARTS>
+__global__ void __launch_bounds__(LOGITS_THREADS, 6)
+logits_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_t grad_stride, T* dlogits, int64_t dlogits_stride, float* dbias) {
+    __shared__ uint16_t listed[SEEN ? LOGITS_WARPS : 1][LOGITS_PART * PARTS];
+    const int lane = threadIdx.x & 31;
+    const int base = blockIdx.x * LOGITS_PART * PARTS, left = a.width - base;
 #pragma unroll 1
-    for (; rows > 0; --rows) {
-        uint32_t ok[LOGITS_PARTS], hit[LOGITS_PARTS];
-        Raw8<T> x[LOGITS_PARTS];
-        Raw8<G> raw[LOGITS_PARTS];
+    for (int row = blockIdx.y * LOGITS_WARPS + (threadIdx.x >> 5); row < a.n_rows; row += gridDim.y * LOGITS_WARPS) {
+        const G* g_row = grad + (row * grad_stride + base);
+        Raw8<G> raw[PARTS];
 #pragma unroll
-        for (int u = 0; u < LOGITS_PARTS; ++u) {
-            ok[u] = tile_bits<MAP>(next.ok, u, lane) & all[u];
-            hit[u] = tile_bits<MAP>(next.hit, u, lane) & ok[u];
+        for (int u = 0; u < PARTS; ++u) {
             raw[u] = {};
-            load_tile<MAP>(g_row + u * LOGITS_PART, ok[u], lane, raw[u]);
+            load_tile<MAP>(g_row + u * LOGITS_PART, tile_all<MAP>(left - u * LOGITS_PART, lane), lane, raw[u]);
         }
+        const uint32_t ok = a.allowed ? tile_word<PARTS>(a.allowed + (row * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
+        const uint32_t hits = SEEN ? tile_hits<PARTS>(a, history_of(a, row), ok, base, left, lane) : 0;
+        T* d_row = dlogits ? dlogits + (row * dlogits_stride + base) : nullptr;
 #pragma unroll
-        for (int u = 0; u < LOGITS_PARTS; ++u) {
-            x[u] = {};
-            load_tile<MAP>(x_row + u * LOGITS_PART, hit[u], lane, x[u]);
-        }
-        const int64_t here = row;
-        row += LOGITS_WARPS;
-        if (rows > 1) next.fetch(a, row, rows > 2, left, lane);
-#pragma unroll
-        for (int u = 0; u < LOGITS_PARTS; ++u) {
+        for (int u = 0; u < PARTS; ++u) {
+            const uint32_t all = tile_all<MAP>(left - u * LOGITS_PART, lane), may = tile_bits<MAP>(ok, u, lane);
             float g[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                g[j] = ok[u] >> j & 1 ? as_float(raw[u].v[j]) : 0.f;
-                if (SHARED) acc[u][j] += g[j];
+            for (int j = 0; j < 8; ++j) g[j] = may >> j & 1 ? as_float(raw[u].v[j]) : 0.f;
+            if (dbias) store_tile<MAP>(dbias + ((int64_t)row * a.width + base + u * LOGITS_PART), all, lane, g);
+            if (d_row) store_tile<MAP>(d_row + u * LOGITS_PART, all, lane, g);
+        }
+        if (SEEN) mend_gradient<PARTS>(a, row, hits, listed[threadIdx.x >> 5], logits + (row * a.stride + base), g_row, d_row, lane);
+    }
+}
+
+// The same with the gradient of a bias that all rows share: a block keeps one tile of columns for rows_per_block rows, each
+// warp adds up every eighth of them in registers, the warps' sums are joined in shared memory, those of several blocks by
+// bias_gradient_kernel.  The incoming gradient is read once for both, and the order of the additions depends on the sizes
+// alone.
+template <typename T, typename G, int MAP, bool SEEN, int PARTS>
+__global__ void __launch_bounds__(LOGITS_THREADS, sizeof(G) == 2 ? 4 : 3)
+logits_bias_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_t grad_stride, T* dlogits, int64_t dlogits_stride,
+                            float* sums, int rows_per_block) {
+    constexpr int R = 2;                                      // rows under way at a time
+    __shared__ float part[LOGITS_WARPS][LOGITS_PART * PARTS];
+    __shared__ uint16_t listed[SEEN ? LOGITS_WARPS : 1][LOGITS_PART * PARTS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int base = blockIdx.x * LOGITS_PART * PARTS, left = a.width - base;
+    const int first = blockIdx.y * rows_per_block, last = a.n_rows - first < rows_per_block ? a.n_rows : first + rows_per_block;
+    float acc[PARTS][8] = {};
+#pragma unroll 1
+    for (int row = first + warp; row < last; row += LOGITS_WARPS * R) {
+        Raw8<G> raw[R][PARTS];
+        uint32_t ok[R], hits[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int i = row + k * LOGITS_WARPS;
+            ok[k] = hits[k] = 0;
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) raw[k][u] = {};
+            if (i < last) {
+#pragma unroll
+                for (int u = 0; u < PARTS; ++u)
+                    load_tile<MAP>(grad + (i * grad_stride + base + u * LOGITS_PART), tile_all<MAP>(left - u * LOGITS_PART, lane), lane, raw[k][u]);
+                ok[k] = a.allowed ? tile_word<PARTS>(a.allowed + (i * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
+                if (SEEN && dlogits) hits[k] = tile_hits<PARTS>(a, history_of(a, i), ok[k], base, left, lane);
             }
-            if (!SHARED && dbias) store_tile<MAP>(dbias + here * a.width + base + u * LOGITS_PART, all[u], lane, g);
-            if (!d_row) continue;
-            if (hit[u]) {
-                const Penalty pen = penalty_of(of_row(a.d_repetition, a.repetition, here));
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int i = row + k * LOGITS_WARPS;
+            if (i >= last) break;
+            T* d_row = dlogits ? dlogits + (i * dlogits_stride + base) : nullptr;
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) {
+                const uint32_t may = tile_bits<MAP>(ok[k], u, lane);
+                float g[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float z = g[j] * (as_float(x[u].v[j]) > 0.f ? pen.up : pen.down);
-                    g[j] = hit[u] >> j & 1 ? z : g[j];
+                    g[j] = may >> j & 1 ? as_float(raw[k][u].v[j]) : 0.f;
+                    acc[u][j] += g[j];
                 }
+                if (d_row) store_tile<MAP>(d_row + u * LOGITS_PART, tile_all<MAP>(left - u * LOGITS_PART, lane), lane, g);
             }
-            store_tile<MAP>(d_row + u * LOGITS_PART, all[u], lane, g);
+            if (SEEN) mend_gradient<PARTS>(a, i, hits[k], listed[warp], logits + (i * a.stride + base), grad + (i * grad_stride + base), d_row, lane);
         }
-        x_row += a.stride * LOGITS_WARPS;
-        g_row += grad_stride * LOGITS_WARPS;
-        if (d_row) d_row += dlogits_stride * LOGITS_WARPS;
     }
-    if (SHARED) {
-        __shared__ float part[LOGITS_WARPS][LOGITS_TILE];
 #pragma unroll
-        for (int u = 0; u < LOGITS_PARTS; ++u)
+    for (int u = 0; u < PARTS; ++u)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) part[warp][u * LOGITS_PART + tile_column<MAP>(lane, j)] = acc[u][j];
-        __syncthreads();
-        for (int v = threadIdx.x; v < left; v += LOGITS_THREADS) {
-            float sum = 0.f;
+        for (int j = 0; j < 8; ++j) part[warp][u * LOGITS_PART + tile_column<MAP>(lane, j)] = acc[u][j];
+    __syncthreads();
+    for (int v = threadIdx.x; v < LOGITS_PART * PARTS && v < left; v += LOGITS_THREADS) {
+        float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < LOGITS_WARPS; ++w) sum += part[w][v];
-            dbias[(int64_t)blockIdx.y * a.width + base + v] = sum;
-        }
+        for (int w = 0; w < LOGITS_WARPS; ++w) sum += part[w][v];
+        sums[(int64_t)blockIdx.y * a.width + base + v] = sum;
     }
 }
 

@@ -41,21 +41,39 @@ _BITS = {torch.int32: 32, torch.int64: 64}
 Number = Union[float, int, torch.Tensor]
 
 
+# The current stream of a device as a number (the public call builds a Stream object on the way: 2 us instead of 0.1).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _words(width: int) -> int:
     return (width + 31) // 32
 
 
-def _need_cuda(t, what: str) -> None:
+def _device_of(t, what: str) -> int:
+    """The number of a tensor's GPU."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a tensor" % what)
-    if t.device.type != "cuda":
+    d = t.get_device()
+    if d < 0:
         raise RuntimeError("%s must be a CUDA tensor; there is no CPU path" % what)
+    return d
 
 
-def _same_device(t, what: str, device) -> None:
-    _need_cuda(t, what)
-    if t.device != device:
-        raise ValueError("%s is on %s, the call on %s" % (what, t.device, device))
+def _on(t, what: str, dev: int) -> None:
+    d = _device_of(t, what)
+    if d != dev:
+        raise ValueError("%s is on cuda:%d, the call on cuda:%d" % (what, d, dev))
+
+
+def _call(fn, dev: int, *args) -> None:
+    """A C entry point with the device current and its current stream as the last argument."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _cabi.check(rc)
 
 
 def _written(t: torch.Tensor) -> None:
@@ -64,30 +82,13 @@ def _written(t: torch.Tensor) -> None:
         torch.autograd.graph.increment_version(t)
 
 
-class _On:
-    """The current stream of a device, with the device current."""
-    __slots__ = ("guard", "stream")
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-        self.stream = torch.cuda.current_stream(device).cuda_stream
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
-
-
-def _tokens(t, what: str, n: int, device) -> torch.Tensor:
-    """[n] whole numbers, int32 or int64, contiguous."""
-    _same_device(t, what, device)
-    if t.dtype not in _BITS or tuple(t.shape) != (n,) or (n > 1 and t.stride(0) != 1):
+def _tokens(t, what: str, n: int, dev: int) -> int:
+    """[n] whole numbers, int32 or int64, contiguous: their bits."""
+    _on(t, what, dev)
+    bits = _BITS.get(t.dtype)
+    if bits is None or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         raise ValueError("%s must be a contiguous int32 or int64 tensor [%d]" % (what, n))
-    return t
+    return bits
 
 
 # --------------------------------------------------------------------------- history
@@ -106,83 +107,90 @@ class TokenHistory:
             raise RuntimeError("a history is kept in CUDA tensors; there is no CPU path")
         words = _words(width)
         self.n_rows, self.width = n_rows, width
+        self.counts: Optional[torch.Tensor] = None
         if counts:                                   # one array, cleared at once: the words, then the counts
             split = (n_rows * words + 3) // 4 * 4
             both = torch.zeros(split + n_rows * width, dtype=torch.int32, device=device)
-            self.seen = both[:n_rows * words].view(n_rows, words)
-            self.counts = both[split:].view(n_rows, width)
+            self.seen = both.as_strided((n_rows, words), (words, 1))
+            self.counts = both.as_strided((n_rows, width), (width, 1), split)
         else:
             self.seen = torch.zeros((n_rows, words), dtype=torch.int32, device=device)
-            self.counts: Optional[torch.Tensor] = None
-        self.device = self.seen.device
+
+    @property
+    def device(self) -> torch.device:
+        return self.seen.device
 
     def clear(self) -> None:
         self.seen.zero_()
         if self.counts is not None:
             self.counts.zero_()
 
-    def _check(self) -> None:
-        for t, what, shape in ((self.seen, "seen", (self.n_rows, _words(self.width))), (self.counts, "counts", (self.n_rows, self.width))):
-            if t is None:
-                continue
-            _same_device(t, what, self.device)
-            if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-                raise ValueError("%s must be a contiguous int32 tensor %r" % (what, shape))
+    def _check(self) -> int:
+        """The number of its GPU."""
+        seen, counts = self.seen, self.counts
+        dev = _device_of(seen, "seen")
+        if seen.dtype is not torch.int32 or seen.shape != (self.n_rows, _words(self.width)) or not seen.is_contiguous():
+            raise ValueError("seen must be a contiguous int32 tensor [%d, %d]" % (self.n_rows, _words(self.width)))
+        if counts is not None:
+            _on(counts, "counts", dev)
+            if counts.dtype is not torch.int32 or counts.shape != (self.n_rows, self.width) or not counts.is_contiguous():
+                raise ValueError("counts must be a contiguous int32 tensor [%d, %d]" % (self.n_rows, self.width))
+        return dev
 
     def add(self, ids, lengths=None, *, offsets=None, pad_left: bool = False, generated: bool = False, rows=None) -> None:
         """Enter the ids of whole rows.  ``ids`` int32 or int64: padded rows [n, T] with their ``lengths`` (int32 [n]; all
         columns without) and the padding on the right unless ``pad_left``, or flat ids with ``offsets`` (int64 [n + 1]): the
         encoder's two layouts.  ``generated``: the row produced them itself, so they are counted too.  ``rows`` [n]: the
         history row of each (0, 1, ... by default).  Ids outside the vocabulary are no tokens."""
-        self._check()
-        _same_device(ids, "ids", self.device)
+        dev = self._check()
+        _on(ids, "ids", dev)
         if ids.dtype not in _BITS:
             raise ValueError("ids must be int32 or int64")
         h = _cabi.History()
         if offsets is not None:
             if lengths is not None or pad_left:
                 raise ValueError("flat ids have offsets, padded rows lengths and a side")
-            _same_device(offsets, "offsets", self.device)
+            _on(offsets, "offsets", dev)
             if ids.dim() != 1 or not ids.is_contiguous():
                 raise ValueError("flat ids must be a contiguous tensor [total]")
-            if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.shape[0] < 1 or not offsets.is_contiguous():
+            if offsets.dtype is not torch.int64 or offsets.dim() != 1 or offsets.shape[0] < 1 or not offsets.is_contiguous():
                 raise ValueError("offsets must be a contiguous int64 tensor [n + 1]")
             n = offsets.shape[0] - 1
             h.offsets, h.total = offsets.data_ptr(), ids.shape[0]
         else:
             if ids.dim() != 2 or (ids.shape[1] > 1 and ids.stride(1) != 1):
                 raise ValueError("padded ids must be a tensor [n, T] whose rows are contiguous")
-            n = ids.shape[0]
-            h.columns, h.id_stride = ids.shape[1], ids.stride(0)
+            n, h.columns = ids.shape
+            h.id_stride = ids.stride(0)
             if lengths is not None:
-                _same_device(lengths, "lengths", self.device)
-                if lengths.dtype != torch.int32 or tuple(lengths.shape) != (n,) or not lengths.is_contiguous():
+                _on(lengths, "lengths", dev)
+                if lengths.dtype is not torch.int32 or lengths.shape != (n,) or not lengths.is_contiguous():
                     raise ValueError("lengths must be a contiguous int32 tensor [%d]" % n)
                 h.lengths = lengths.data_ptr()
             h.pad_left = 1 if pad_left else 0
-        self._enter(h, ids, n, rows, generated)
+        self._enter(h, ids, n, rows, generated, dev)
 
     def append(self, tokens, rows=None) -> None:
         """Enter one generated token per row: ``tokens`` [n] int32 or int64; ``rows`` as in ``add``.  A token outside the
         vocabulary (-1, say) is none."""
-        self._check()
+        dev = self._check()
         n = tokens.shape[0] if isinstance(tokens, torch.Tensor) and tokens.dim() == 1 else 0
-        _tokens(tokens, "tokens", n, self.device)
+        _tokens(tokens, "tokens", n, dev)
         h = _cabi.History()
         h.columns = h.id_stride = 1
-        self._enter(h, tokens, n, rows, True)
+        self._enter(h, tokens, n, rows, True, dev)
 
-    def _enter(self, h, ids, n: int, rows, generated: bool) -> None:
+    def _enter(self, h, ids, n: int, rows, generated: bool, dev: int) -> None:
         if rows is not None:
-            h.rows, h.rows_bits = _tokens(rows, "rows", n, self.device).data_ptr(), _BITS[rows.dtype]
+            h.rows_bits = _tokens(rows, "rows", n, dev)
+            h.rows = rows.data_ptr()
         elif n != self.n_rows:
             raise ValueError("the history has %d rows, the call %d" % (self.n_rows, n))
         h.seen, h.history_rows, h.width = self.seen.data_ptr(), self.n_rows, self.width
         if self.counts is not None:
             h.counts = self.counts.data_ptr()
         h.ids, h.id_bits, h.n_rows = ids.data_ptr(), _BITS[ids.dtype], n
-        with _On(self.device) as stream:
-            _cabi.check(_cabi.lib().dnatok_history_add(ctypes.byref(h), 1 if generated else 0, stream))
+        _call(_cabi.lib().dnatok_history_add, dev, h, 1 if generated else 0)
         _written(self.seen)
         if generated and self.counts is not None:
             _written(self.counts)
@@ -241,27 +249,35 @@ class Grammar:
                           device=torch.device("cuda" if device is None else device))
 
     @staticmethod
-    def _states(states) -> int:
-        _need_cuda(states, "states")
-        if states.dtype != torch.int32 or states.dim() != 1 or (states.shape[0] > 1 and states.stride(0) != 1):
+    def _states(states) -> Tuple[int, int]:
+        dev = _device_of(states, "states")
+        if states.dtype is not torch.int32 or states.dim() != 1 or (states.shape[0] > 1 and states.stride(0) != 1):
             raise ValueError("states must be a contiguous int32 tensor [n]")
-        return states.shape[0]
+        return states.shape[0], dev
 
-    def _mask(self, n: int, device, out):
-        shape = (n, _words(self.width))
+    def _mask(self, states, n: int, dev: int, out):
+        words = _words(self.width)
         if out is None:
-            return torch.empty(shape, dtype=torch.int32, device=device)
-        _same_device(out, "the mask", device)
-        if out.dtype != torch.int32 or tuple(out.shape) != shape or not out.is_contiguous():
-            raise ValueError("the mask must be a contiguous int32 tensor %r" % (shape,))
+            return states.new_empty((n, words))
+        _on(out, "the mask", dev)
+        if out.dtype is not torch.int32 or out.shape != (n, words) or not out.is_contiguous():
+            raise ValueError("the mask must be a contiguous int32 tensor [%d, %d]" % (n, words))
+        return out
+
+    @staticmethod
+    def _new_states(states, n: int, dev: int, out):
+        if out is None:
+            return states.new_empty((n,))
+        _on(out, "out", dev)
+        if out.dtype is not torch.int32 or out.shape != (n,) or not out.is_contiguous():
+            raise ValueError("out must be a contiguous int32 tensor [%d]" % n)
         return out
 
     def allowed(self, states, *, out=None) -> torch.Tensor:
         """int32 [n, words]: the tokens that may follow in each state."""
-        n = self._states(states)
-        mask = self._mask(n, states.device, out)
-        with _On(states.device) as stream:
-            _cabi.check(_cabi.lib().dnatok_grammar_allowed(self.ptr, states.data_ptr(), n, mask.data_ptr(), stream))
+        n, dev = self._states(states)
+        mask = self._mask(states, n, dev, out)
+        _call(_cabi.lib().dnatok_grammar_allowed, dev, self.ptr, states.data_ptr(), n, mask.data_ptr())
         if out is not None:
             _written(out)
         return mask
@@ -269,39 +285,26 @@ class Grammar:
     def advance(self, states, tokens, *, out=None) -> torch.Tensor:
         """int32 [n]: the states after ``tokens`` [n] (int32 or int64); a token outside the vocabulary (-1, say) leaves its
         row as it was.  ``out`` may be ``states``."""
-        n = self._states(states)
-        _tokens(tokens, "tokens", n, states.device)
-        new = self._new_states(n, states.device, out)
-        with _On(states.device) as stream:
-            _cabi.check(_cabi.lib().dnatok_grammar_step(self.ptr, states.data_ptr(), tokens.data_ptr(), _BITS[tokens.dtype], n,
-                                                        new.data_ptr(), None, stream))
+        n, dev = self._states(states)
+        bits = _tokens(tokens, "tokens", n, dev)
+        new = self._new_states(states, n, dev, out)
+        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, states.data_ptr(), tokens.data_ptr(), bits, n, new.data_ptr(), None)
         if out is not None:
             _written(out)
         return new
 
     def step(self, states, tokens, *, out=None, out_allowed=None) -> Tuple[torch.Tensor, torch.Tensor]:
         """``advance`` and the masks of the new states in one call: (states, allowed).  ``out`` may not be ``states``."""
-        n = self._states(states)
-        _tokens(tokens, "tokens", n, states.device)
-        new = self._new_states(n, states.device, out)
-        mask = self._mask(n, states.device, out_allowed)
-        with _On(states.device) as stream:
-            _cabi.check(_cabi.lib().dnatok_grammar_step(self.ptr, states.data_ptr(), tokens.data_ptr(), _BITS[tokens.dtype], n,
-                                                        new.data_ptr(), mask.data_ptr(), stream))
+        n, dev = self._states(states)
+        bits = _tokens(tokens, "tokens", n, dev)
+        new = self._new_states(states, n, dev, out)
+        mask = self._mask(states, n, dev, out_allowed)
+        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, states.data_ptr(), tokens.data_ptr(), bits, n, new.data_ptr(), mask.data_ptr())
         if out is not None:
             _written(out)
         if out_allowed is not None:
             _written(out_allowed)
         return new, mask
-
-    @staticmethod
-    def _new_states(n: int, device, out):
-        if out is None:
-            return torch.empty(n, dtype=torch.int32, device=device)
-        _same_device(out, "out", device)
-        if out.dtype != torch.int32 or tuple(out.shape) != (n,) or not out.is_contiguous():
-            raise ValueError("out must be a contiguous int32 tensor [%d]" % n)
-        return out
 
 
 # --------------------------------------------------------------------------- logits
@@ -311,40 +314,59 @@ def _rows_of(t: torch.Tensor, what: str) -> None:
         raise ValueError("%s must be a tensor [n, width] whose rows are contiguous" % what)
 
 
-def _penalty(a, name: str, v, n: int, device, keep: list) -> bool:
-    """Enters one penalty; whether it is one."""
+def _penalty(name: str, v, n: int, dev: int):
+    """(number, address of one value a row, whether it is a penalty)."""
     neutral = 1.0 if name == "repetition" else 0.0
     if isinstance(v, torch.Tensor):
-        _same_device(v, name, device)
-        if v.dtype != torch.float32 or tuple(v.shape) != (n,) or (n > 1 and v.stride(0) != 1):
+        _on(v, name, dev)
+        if v.dtype is not torch.float32 or v.shape != (n,) or (n > 1 and v.stride(0) != 1):
             raise ValueError("%s must be a number or a contiguous float32 tensor [%d]" % (name, n))
         if v.requires_grad and torch.is_grad_enabled():
             raise ValueError("%s has no gradient" % name)
-        setattr(a, "d_" + name, v.data_ptr())
-        setattr(a, name, neutral)
-        keep.append(v)
-        return True
+        return neutral, v.data_ptr(), True
     v = float(v)
-    if name == "repetition" and not 2.0 ** -126 <= v <= 2.0 ** 126:
-        raise ValueError("repetition must be positive and finite (2^-126 to 2^126)")
-    if v != v or v in (float("inf"), -float("inf")):
+    if name == "repetition":
+        if not 2.0 ** -126 <= v <= 2.0 ** 126:
+            raise ValueError("repetition must be positive and finite (2^-126 to 2^126)")
+    elif v - v != 0.0:
         raise ValueError("%s must be finite" % name)
-    setattr(a, name, v)
-    return v != neutral
+    return v, None, v != neutral
+
+
+def _shared(t) -> bool:
+    """Whether an array of one row, or without rows, stands for all of them."""
+    return t.dim() == 1 or t.shape[0] == 1
+
+
+def _row_array(t, what: str, dtype, n: int, columns: int, dev: int) -> Tuple[int, int]:
+    """(address, elements from row to row) of an array [columns], [1, columns] or [n, columns]; 0 elements where one row stands
+    for all."""
+    _on(t, what, dev)
+    shape, strides = t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) not in (1, 2) or shape[-1] != columns or (columns > 1 and strides[-1] != 1) \
+            or (len(shape) == 2 and shape[0] != 1 and shape[0] != n):
+        raise ValueError("%s must be a %s tensor [%d, %d] or [%d] whose rows are contiguous" % (what, str(dtype)[6:], n, columns, columns))
+    if len(shape) == 1 or shape[0] == 1:
+        return t.data_ptr(), 0
+    if strides[0] < columns:
+        raise ValueError("rows of %s overlap" % what)
+    return t.data_ptr(), strides[0]
 
 
 def _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed):
-    """(the C arguments, tensors whose addresses they hold)."""
-    _need_cuda(logits, "logits")
+    """(the C arguments, the number of the GPU)."""
+    dev = _device_of(logits, "logits")
     _rows_of(logits, "logits")
-    if logits.dtype not in _TYPES:
+    dtype = _TYPES.get(logits.dtype)
+    if dtype is None:
         raise ValueError("logits must be float32, float16 or bfloat16")
     n, width = logits.shape
-    device = logits.device
-    a, keep = _cabi.Logits(), [logits]
-    a.logits, a.dtype, a.n_rows, a.width, a.stride = logits.data_ptr(), _TYPES[logits.dtype], n, width, logits.stride(0)
-    once = _penalty(a, "repetition", repetition, n, device, keep)
-    often = _penalty(a, "frequency", frequency, n, device, keep) | _penalty(a, "presence", presence, n, device, keep)
+    a = _cabi.Logits()
+    a.logits, a.dtype, a.n_rows, a.width, a.stride = logits.data_ptr(), dtype, n, width, logits.stride(0)
+    a.repetition, a.d_repetition, once = _penalty("repetition", repetition, n, dev)
+    a.frequency, a.d_frequency, often = _penalty("frequency", frequency, n, dev)
+    a.presence, a.d_presence, also = _penalty("presence", presence, n, dev)
+    often = often or also
     if history is None:
         if once or often:
             raise ValueError("penalties need a history")
@@ -353,89 +375,70 @@ def _arguments(logits, history, rows, repetition, frequency, presence, bias, all
     else:
         if history.width != width:
             raise ValueError("the history has %d tokens, the logits %d" % (history.width, width))
-        history._check()
-        if history.device != device:
-            raise ValueError("the history is on %s, the logits on %s" % (history.device, device))
+        if history._check() != dev:
+            raise ValueError("the history is on %s, the logits on %s" % (history.device, logits.device))
         if rows is not None:
-            a.rows, a.rows_bits = _tokens(rows, "rows", n, device).data_ptr(), _BITS[rows.dtype]
-            keep.append(rows)
+            a.rows_bits = _tokens(rows, "rows", n, dev)
+            a.rows = rows.data_ptr()
         elif history.n_rows != n:
             raise ValueError("the history has %d rows, the logits %d" % (history.n_rows, n))
         if often and history.counts is None:
             raise ValueError("frequency and presence need a history that keeps counts")
         if once or often:
             a.seen, a.history_rows = history.seen.data_ptr(), history.n_rows
-            keep.append(history.seen)
         if often:
             a.counts = history.counts.data_ptr()
-            keep.append(history.counts)
     if bias is not None:
-        _same_device(bias, "bias", device)
-        if bias.dtype != torch.float32 or tuple(bias.shape) not in ((width,), (1, width), (n, width)) or (width > 1 and bias.stride(-1) != 1):
-            raise ValueError("bias must be a float32 tensor [%d] or [%d, %d] whose rows are contiguous" % (width, n, width))
-        shared = bias.dim() == 1 or bias.shape[0] == 1
-        if not shared and bias.stride(0) < width:
-            raise ValueError("rows of the bias overlap")
-        a.bias, a.bias_stride = bias.data_ptr(), 0 if shared else bias.stride(0)
-        keep.append(bias)
+        a.bias, a.bias_stride = _row_array(bias, "bias", torch.float32, n, width, dev)
     if allowed is not None:
-        words = _words(width)
-        _same_device(allowed, "allowed", device)
-        if allowed.dtype != torch.int32 or tuple(allowed.shape) not in ((words,), (1, words), (n, words)) or (words > 1 and allowed.stride(-1) != 1):
-            raise ValueError("allowed must be an int32 tensor [%d, %d] or [%d] whose rows are contiguous" % (n, words, words))
-        shared = allowed.dim() == 1 or allowed.shape[0] == 1
-        if not shared and allowed.stride(0) < words:
-            raise ValueError("rows of the mask overlap")
-        a.allowed, a.allowed_stride = allowed.data_ptr(), 0 if shared else allowed.stride(0)
-        keep.append(allowed)
-    return a, keep
+        a.allowed, a.allowed_stride = _row_array(allowed, "allowed", torch.int32, n, _words(width), dev)
+    return a, dev
 
 
 def _output(logits, out, out_dtype):
     dtype = out_dtype or (logits.dtype if out is None else out.dtype)
-    if dtype not in (logits.dtype, torch.float32):
+    if dtype is not logits.dtype and dtype is not torch.float32:
         raise ValueError("the output has the logits' type or is float32")
     if out is None:
-        return torch.empty(logits.shape, dtype=dtype, device=logits.device)
-    _same_device(out, "out", logits.device)
+        if dtype is logits.dtype and logits.is_contiguous():
+            return torch.empty_like(logits)                        # (the quickest of the two calls)
+        return logits.new_empty(logits.shape, dtype=dtype)
+    _on(out, "out", logits.get_device())
     _rows_of(out, "out")
-    if out.dtype != dtype or out.shape != logits.shape:
+    if out.dtype is not dtype or out.shape != logits.shape:
         raise ValueError("out must be a %s tensor %r" % (dtype, tuple(logits.shape)))
     return out
 
 
-def _forward(a, logits, out):
-    with _On(logits.device) as stream:
-        _cabi.check(_cabi.lib().dnatok_process_logits(ctypes.byref(a), out.data_ptr(), _TYPES[out.dtype], out.stride(0), stream))
+def _forward(a, dev: int, out):
+    _call(_cabi.lib().dnatok_process_logits, dev, a, out.data_ptr(), _TYPES[out.dtype], out.stride(0))
     return out
 
 
-def _backward(a, logits, grad, bias_shape, want_logits: bool, want_bias: bool):
+def _backward(a, dev: int, logits, grad, bias, want_logits: bool, want_bias: bool):
     if grad.shape[1] > 1 and grad.stride(1) != 1:
         grad = grad.contiguous()
     n, width = grad.shape
-    dx = torch.empty((n, width), dtype=logits.dtype, device=grad.device) if want_logits else None
-    db = scratch = None
-    need = 0
     L = _cabi.lib()
-    with _On(grad.device) as stream:
-        if want_bias:
-            db = torch.empty(bias_shape, dtype=torch.float32, device=grad.device)
-            need = L.dnatok_logits_scratch_bytes(n, width) if a.bias_stride == 0 else 0
+    dx = logits.new_empty((n, width)) if want_logits else None
+    db, scratch, need = None, None, 0
+    if want_bias:
+        db = bias.new_empty(bias.shape)
+        if a.bias_stride == 0:
+            need = L.dnatok_logits_scratch_bytes(n, width)
             if need:
-                scratch = torch.empty(need, dtype=torch.uint8, device=grad.device)
-        _cabi.check(L.dnatok_process_logits_backward(
-            ctypes.byref(a), grad.data_ptr(), _TYPES[grad.dtype], grad.stride(0), dx.data_ptr() if dx is not None else None,
-            dx.stride(0) if dx is not None else 0, db.data_ptr() if db is not None else None,
-            scratch.data_ptr() if scratch is not None else None, need, stream))
+                scratch = logits.new_empty((need,), dtype=torch.uint8)
+    _call(L.dnatok_process_logits_backward, dev, a, grad.data_ptr(), _TYPES[grad.dtype], grad.stride(0),
+          dx.data_ptr() if dx is not None else None, width, db.data_ptr() if db is not None else None,
+          scratch.data_ptr() if need else None, need)
     return dx, db
 
 
 class _Process(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, history, rows, repetition, frequency, presence, allowed, out_dtype):
-        a, _ = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
-        out = _forward(a, logits, _output(logits, None, out_dtype))
+        a, dev = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
+        out = _forward(a, dev, _output(logits, None, out_dtype))
         ctx.save_for_backward(logits, bias, rows if a.rows else None, allowed, history.seen if a.seen else None,
                               repetition if isinstance(repetition, torch.Tensor) else None)
         ctx.number = a.repetition
@@ -457,11 +460,10 @@ class _Process(torch.autograd.Function):
         if rows is not None:
             a.rows, a.rows_bits = rows.data_ptr(), _BITS[rows.dtype]
         if allowed is not None:
-            a.allowed, a.allowed_stride = allowed.data_ptr(), 0 if allowed.dim() == 1 or allowed.shape[0] == 1 else allowed.stride(0)
-        if bias is not None and bias.dim() == 2 and bias.shape[0] != 1:
-            a.bias_stride = bias.stride(0)
-        dx, db = _backward(a, logits, grad, bias.shape if bias is not None else None, ctx.needs_input_grad[0],
-                           ctx.needs_input_grad[1])
+            a.allowed, a.allowed_stride = allowed.data_ptr(), 0 if _shared(allowed) else allowed.stride(0)
+        if bias is not None and not _shared(bias):
+            a.bias_stride = a.width
+        dx, db = _backward(a, logits.get_device(), logits, grad, bias, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dx, db, None, None, None, None, None, None, None
 
 
@@ -479,13 +481,12 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
 
     All of it is computed in 32 bits and rounded once.  Differentiable in ``logits`` and ``bias``; the history and the mask
     must then stay as they are until the backward pass (autograd refuses it otherwise)."""
-    if torch.is_grad_enabled() and ((isinstance(logits, torch.Tensor) and logits.requires_grad)
-                                    or (isinstance(bias, torch.Tensor) and bias.requires_grad)):
+    if torch.is_grad_enabled() and (getattr(logits, "requires_grad", False) or getattr(bias, "requires_grad", False)):
         if out is not None:
             raise ValueError("out= has no gradient; leave it out or call under torch.no_grad()")
         return _Process.apply(logits, bias, history, rows, repetition, frequency, presence, allowed, out_dtype)
-    a, _ = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
-    result = _forward(a, logits, _output(logits, out, out_dtype))
+    a, dev = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
+    result = _forward(a, dev, _output(logits, out, out_dtype))
     if out is not None:
         _written(out)
     return result
@@ -496,8 +497,10 @@ def process_logits_backward(grad, logits, *, history: Optional[TokenHistory] = N
     """(gradient of ``logits``, gradient of ``bias`` or None) for ``grad``, the gradient of ``process_logits`` called with the
     same arguments; without autograd."""
     with torch.no_grad():
-        a, _ = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
-        _same_device(grad, "grad", logits.device)
+        a, dev = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
+        _on(grad, "grad", dev)
         if grad.dim() != 2 or grad.shape != logits.shape or grad.dtype not in (logits.dtype, torch.float32):
             raise ValueError("grad must be a tensor %r of the logits' type or float32" % (tuple(logits.shape),))
-        return _backward(a, logits, grad, bias.shape if bias is not None else None, True, bias is not None)
+        if bias is not None and not _shared(bias):
+            a.bias_stride = a.width
+        return _backward(a, dev, logits, grad, bias, True, bias is not None)
