@@ -333,8 +333,9 @@ struct dnatok_grammar {
     std::vector<uint64_t> text;
     std::vector<uint32_t> super;
     std::vector<uint2> prefix;
-    std::vector<uint4> rest;
-    int32_t n_states = 0, log_pitch = 0, n_groups = 0, super_steps = 0, prefix_steps = 0;
+    std::vector<uint2> rest;
+    std::vector<uint32_t> more;
+    int32_t n_states = 0, log_pitch = 0, n_groups = 0, super_steps = 0, prefix_steps = 0, n_runs = 0;
     int64_t width = 0, end_id = -1;
     struct Device { void* memory = nullptr; GrammarTables tables{}; };
     std::mutex mu;
@@ -356,11 +357,11 @@ int grammar_tables(dnatok_grammar* g, cudaStream_t stream, GrammarTables* out) {
         CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
         if (capturing != cudaStreamCaptureStatusNone)
             return abi_fail(DNATOK_ERR_INVALID, "a grammar's first use on a device must be outside of stream capture");
-        constexpr int N = 10;
+        constexpr int N = 11;
         const size_t sizes[N] = {g->next.size() * 4, g->step16.size() * 2, g->accepting.size(), g->codes.size(), g->token_at.size() * 4,
-                                 g->text.size() * 8, g->prefix.size() * 8, g->rest.size() * 16, g->step32.size() * 4, g->super.size() * 4};
+                                 g->text.size() * 8, g->prefix.size() * 8, g->rest.size() * 8, g->step32.size() * 4, g->super.size() * 4, g->more.size() * 4};
         const void* from[N] = {g->next.data(), g->step16.data(), g->accepting.data(), g->codes.data(), g->token_at.data(),
-                               g->text.data(), g->prefix.data(), g->rest.data(), g->step32.data(), g->super.data()};
+                               g->text.data(), g->prefix.data(), g->rest.data(), g->step32.data(), g->super.data(), g->more.data()};
         size_t at[N + 1] = {0};
         for (int i = 0; i < N; ++i) at[i + 1] = at[i] + up256(sizes[i] + 1);
         struct Undo {
@@ -385,9 +386,11 @@ int grammar_tables(dnatok_grammar* g, cudaStream_t stream, GrammarTables* out) {
         t.text = g->text.empty() ? nullptr : (const uint64_t*)(base + at[5]);
         t.prefix = (const uint2*)(base + at[6]);
         t.super = (const uint32_t*)(base + at[9]);
-        t.rest = (const uint4*)(base + at[7]);
+        t.rest = (const uint2*)(base + at[7]);
+        t.more = (const uint32_t*)(base + at[10]);
         t.n_states = g->n_states; t.log_pitch = g->log_pitch; t.n_groups = g->n_groups;
         t.n_super = (int32_t)g->super.size();
+        t.n_runs = g->n_runs;
         t.super_steps = g->super_steps; t.prefix_steps = g->prefix_steps;
         t.width = g->width; t.end_id = g->end_id;
         d.memory = undo.memory;
@@ -421,12 +424,15 @@ int launch_allowed(const GrammarTables& t, const int32_t* states, const void* to
         LAUNCH_CHECK("grammar_any_kernel");
         return DNATOK_OK;
     }
-    // A warp for every 4 groups, up to 8 where rows fill the GPU, else up to 16.  Few rows: up to 8 blocks a row, as long as
-    // all are on the GPU at once and each of their warps has 4 groups.
+    // Few rows: up to 8 blocks a row, as long as all are on the GPU at once (3 an SM) and each has 128 groups.  A warp for
+    // every 4 groups, up to 16; 8 where rows fill the GPU by themselves.  (1,024 rows of a pattern over 32,000 tokens: 31 us
+    // with 8, 54 with 4, because the rows differ and one that may go on with anything holds up the rest; 148 such rows: 20 us
+    // in 296 blocks, 25 in 592, which are two rounds.)
+    const int64_t room = (int64_t)SMS * 3;
     int parts = 1;
-    while (parts < 8 && n_rows * parts * 2 <= SMS * 4 && t.n_groups > parts * 128) parts *= 2;
+    while (parts < 8 && n_rows * parts * 2 <= room && t.n_groups > parts * 128) parts *= 2;
     int warps = 1;
-    const int most = n_rows > SMS * 4 ? 8 : GRAMMAR_MOST / 32;
+    const int most = n_rows > room ? 8 : GRAMMAR_MOST / 32;
     while (warps < most && warps * 4 * parts < t.n_groups) warps *= 2;
     int split = 1;                                            // warps a set of 32 groups
     while (split < 32 && split < warps * parts && t.n_super * split < warps * parts) split *= 2;
@@ -443,11 +449,12 @@ int launch_allowed(const GrammarTables& t, const int32_t* states, const void* to
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
     cudaError_t e = cudaSuccess;
-    auto run = [&](auto s, auto n, auto c) {
-        e = cudaLaunchKernelEx(&cfg, grammar_allowed_kernel<decltype(s), decltype(n)::value, decltype(c)::value>, t, states, tokens,
-                               token_bits, states_out, allowed, parts, split);
+    auto run = [&](auto s, auto n, auto c, auto r) {
+        e = cudaLaunchKernelEx(&cfg, grammar_allowed_kernel<decltype(s), decltype(n)::value, decltype(c)::value, decltype(r)::value>, t,
+                               states, tokens, token_bits, states_out, allowed, parts, split);
     };
-    auto placed = [&](auto s, auto n) { if (parts > 1) run(s, n, std::true_type()); else run(s, n, std::false_type()); };
+    auto marked = [&](auto s, auto n, auto c) { if (t.n_runs * 2 > t.n_groups) run(s, n, c, std::true_type()); else run(s, n, c, std::false_type()); };
+    auto placed = [&](auto s, auto n) { if (parts > 1) marked(s, n, std::true_type()); else marked(s, n, std::false_type()); };
     auto typed = [&](auto s) { if (near) placed(s, std::true_type()); else placed(s, std::false_type()); };
     if (t.step16) typed(uint16_t()); else typed(uint32_t());
     if (e != cudaSuccess) return abi_fail(DNATOK_ERR_CUDA, "launch of grammar_allowed_kernel: %s", cudaGetErrorString(e));
@@ -473,8 +480,12 @@ void sort_tokens(dnatok_grammar* g) {
         if (length(v) && v != g->end_id) order.push_back(v);
     }
     const int64_t mean = order.empty() ? 0 : ((int64_t)g->codes.size() + (int64_t)order.size() - 1) / (int64_t)order.size();
+    std::vector<uint64_t> key((size_t)g->width);              // the first 16 classes, ends first
+    for (int32_t v : order)
+        for (int64_t i = 0; i < 16; ++i) key[(size_t)v] = key[(size_t)v] << 4 | (uint64_t)(i < length(v) ? code(v, i) + 1 : 0);
     std::sort(order.begin(), order.end(), [&](int32_t x, int32_t y) {
         if ((length(x) > mean) != (length(y) > mean)) return length(y) > mean;
+        if (key[(size_t)x] != key[(size_t)y]) return key[(size_t)x] < key[(size_t)y];
         const int64_t n = std::min(length(x), length(y));
         const int c = memcmp(&g->codes[(size_t)g->token_at[(size_t)x]], &g->codes[(size_t)g->token_at[(size_t)y]], (size_t)n);
         return c ? c < 0 : length(x) != length(y) ? length(x) < length(y) : x < y;
@@ -490,7 +501,8 @@ void sort_tokens(dnatok_grammar* g) {
     const size_t sets = (order.size() + 1023) / 1024;
     g->n_groups = (int32_t)((order.size() + 31) / 32);
     g->prefix.assign(sets * 32, make_uint2(0, 0));
-    g->rest.assign(sets * 1024, make_uint4(0, 0, ~0u, 0));
+    g->rest.assign(sets * 1024, make_uint2(0, ~0u));
+    g->more.assign(sets * 1024, 0);
     for (size_t s = 0; s < sets; ++s) {
         const size_t end = std::min(order.size(), (s + 1) * 1024);
         const int64_t m = common(s * 1024, end, 0, GRAMMAR_SHARED);
@@ -500,14 +512,18 @@ void sort_tokens(dnatok_grammar* g) {
             const size_t last = std::min(end, k * 32 + 32);
             const int64_t n = common(k * 32, last, m, GRAMMAR_SHARED);
             int64_t steps = 1;                                // (0 says that there is no group)
+            bool run = true;
             for (size_t i = k * 32; i < last; ++i) {
                 const int32_t v = order[i];
                 steps = std::max(steps, length(v) - m - n);
                 const uint64_t rest = classes(v, m + n, length(v), GRAMMAR_REST);
-                g->rest[i] = make_uint4((uint32_t)rest, (uint32_t)(rest >> 32), (uint32_t)v, 0);
+                g->rest[i] = make_uint2((uint32_t)rest, (uint32_t)v);
+                g->more[i] = (uint32_t)(rest >> 32);
+                run = run && v == order[k * 32] + (int32_t)(i - k * 32);
             }
-            g->prefix[k] = make_uint2((uint32_t)classes(order[k * 32], m, m + n, GRAMMAR_SHARED), (uint32_t)(steps > GRAMMAR_REST ? GRAMMAR_SLOW : steps));
+            g->prefix[k] = make_uint2((uint32_t)classes(order[k * 32], m, m + n, GRAMMAR_SHARED), (uint32_t)(steps > GRAMMAR_REST ? GRAMMAR_SLOW : steps) | (run ? GRAMMAR_RUN : 0));
             g->prefix_steps = std::max(g->prefix_steps, (int32_t)n);
+            g->n_runs += run;
         }
     }
 }

@@ -25,7 +25,7 @@ constexpr int32_t GRAMMAR_DEAD = -1, GRAMMAR_FINISHED = -2;
 constexpr int GRAMMAR_PACKED = 14;
 // What 32 groups share, and a group behind that, has up to 8 classes; a token's rest has up to 16, or its group is walked
 // code by code (GRAMMAR_SLOW).  All are filled up with the class that leaves every state as it is.
-constexpr int GRAMMAR_SHARED = 8, GRAMMAR_REST = 16, GRAMMAR_SLOW = 255;
+constexpr int GRAMMAR_SHARED = 8, GRAMMAR_REST = 16, GRAMMAR_SLOW = 255, GRAMMAR_RUN = 256;
 
 struct GrammarTables {
     const int32_t* next;          // [n_states << log_pitch], -1: no way on
@@ -38,9 +38,11 @@ struct GrammarTables {
     const uint16_t* step16;
     const uint32_t* step32;
     const uint32_t* super;        // [n_super] what 32 groups share
-    const uint2* prefix;          // [n_super * 32] x: what a group shares behind that; y: steps that its tokens take then, 0: no group
-    const uint4* rest;            // [n_super * 1024] x, y: 8 and 8 classes, what each token has behind the prefix; z: its id, -1: none
-    int32_t n_states, log_pitch, n_groups, n_super, super_steps, prefix_steps;
+    const uint2* prefix;          // [n_super * 32] x: what a group shares behind that; y: steps that its tokens take then, 0: no group, and
+                                  // GRAMMAR_RUN if their ids follow one another
+    const uint2* rest;            // [n_super * 1024] x: the first 8 classes that each token has behind the prefix; y: its id, -1: none
+    const uint32_t* more;         // [n_super * 1024] the 8 classes behind those, read for groups that have any
+    int32_t n_states, log_pitch, n_groups, n_super, super_steps, prefix_steps, n_runs;
     int64_t width;
     int64_t end_id;               // -1: none
 };
@@ -114,7 +116,7 @@ constexpr int GRAMMAR_NEAR_BYTES = 16 * 1024;
 
 constexpr int GRAMMAR_MOST = 512;                              // threads a block
 
-template <typename S, bool NEAR, bool CLUSTER>
+template <typename S, bool NEAR, bool CLUSTER, bool RUNS>
 __global__ void __launch_bounds__(GRAMMAR_MOST, 3)
 grammar_allowed_kernel(GrammarTables t, const int32_t* __restrict__ states, const void* __restrict__ tokens, int token_bits,
                        int32_t* __restrict__ states_out, uint32_t* __restrict__ allowed, int parts, int split) {
@@ -172,7 +174,7 @@ grammar_allowed_kernel(GrammarTables t, const int32_t* __restrict__ states, cons
                 sets &= sets - 1;
                 const int g0 = (s0 + k0) * 32;
                 const uint2 group = __ldg(t.prefix + g0 + lane);
-                const int steps_mine = (int)group.y;
+                const int steps_mine = (int)(group.y & 255), run_mine = (int)(group.y & GRAMMAR_RUN);
                 uint32_t mine = __shfl_sync(FULL, of_set, k0);    // state behind the prefix of this lane's group
                 if ((lane & (split - 1)) != __shfl_sync(FULL, share, k0) || steps_mine == 0) mine = dead;
                 uint32_t prefix = group.x;
@@ -182,35 +184,52 @@ grammar_allowed_kernel(GrammarTables t, const int32_t* __restrict__ states, cons
                 uint32_t slow = __ballot_sync(FULL, mine != dead && steps_mine == GRAMMAR_SLOW);
                 auto walk = [&](auto together) {                  // the next groups of `alive`, that many at a time
                     constexpr int N = decltype(together)::value;
-                    uint4 text[N];
+                    uint2 text[N];
+                    int at[N];
                     uint32_t s[N];
-                    int steps = 0;
+                    int run[N], steps = 0;
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
                         const int k = __ffs(alive) - 1;
                         alive &= alive - 1;
-                        text[i] = __ldg(t.rest + ((g0 + k) * 32 + lane));
+                        at[i] = (g0 + k) * 32 + lane;
+                        text[i] = __ldg(t.rest + at[i]);
                         s[i] = __shfl_sync(FULL, mine, k);
                         steps = max(steps, __shfl_sync(FULL, steps_mine, k));
+                        run[i] = RUNS ? __shfl_sync(FULL, run_mine, k) : 0;
                     }
                     for (int n = 0; n < steps; ++n) {
+                        if (n == 8) {
+#pragma unroll
+                            for (int i = 0; i < N; ++i) text[i].x = __ldg(t.more + at[i]);
+                        }
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
-                            if (n == 8) text[i].x = text[i].y;
                             s[i] = step(s[i], text[i].x & 15);
                             text[i].x >>= 4;
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (s[i] != dead && (int)text[i].z >= 0) atomicOr(set + (text[i].z >> 5), 1u << (text[i].z & 31));
+                    for (int i = 0; i < N; ++i) {
+                        const bool ok = s[i] != dead && (int)text[i].y >= 0;
+                        if (RUNS && run[i]) {
+                            const uint32_t word = __ballot_sync(FULL, ok);
+                            const uint32_t at = __shfl_sync(FULL, text[i].y, 0);
+                            if (lane < 2 && word) {
+                                const uint32_t bits = lane == 0 ? word << (at & 31) : (at & 31) ? word >> (32 - (at & 31)) : 0;
+                                if (bits) atomicOr(set + (at >> 5) + lane, bits);
+                            }
+                        } else if (ok) {
+                            atomicOr(set + (text[i].y >> 5), 1u << (text[i].y & 31));
+                        }
+                    }
                 };
                 while (__popc(alive) >= TOGETHER) walk(std::integral_constant<int, TOGETHER>());
                 while (alive) walk(std::integral_constant<int, 1>());
                 while (slow) {                                    // groups with a longer token: from the row's state, code by code
                     const int k = __ffs(slow) - 1;
                     slow &= slow - 1;
-                    const int32_t id = (int32_t)__ldg(&t.rest[(g0 + k) * 32 + lane].z);
+                    const int32_t id = (int32_t)__ldg(&t.rest[(g0 + k) * 32 + lane].y);
                     if (id >= 0 && grammar_walk_codes(t, state, id) >= 0) atomicOr(set + (id >> 5), 1u << (id & 31));
                 }
             }
