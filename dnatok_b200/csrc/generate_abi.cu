@@ -202,6 +202,7 @@ int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, 
     if (in->n_rows && !d_grad) return abi_fail(DNATOK_ERR_INVALID, "gradient is NULL");
     if (!aligned(d_grad, size_of(grad_dtype)) || !aligned(d_dbias, 4)) return abi_fail(DNATOK_ERR_INVALID, "misaligned gradient");
     if (d_dlogits) if (int rc = check_output("logits' gradient", d_dlogits, size_of(in->dtype), dlogits_stride, in)) return rc;
+    if (d_dlogits && d_dlogits == in->logits && in->n_rows) return abi_fail(DNATOK_ERR_INVALID, "the logits are still read: their gradient needs an array of its own");
     if (d_dlogits && d_dlogits == d_grad && in->n_rows && (grad_dtype != in->dtype || (in->n_rows > 1 && grad_stride != dlogits_stride)))
         return abi_fail(DNATOK_ERR_INVALID, "in place both gradients have one type and stride");
     cudaStream_t st = (cudaStream_t)stream;
@@ -260,16 +261,20 @@ template <typename IdT>
 int launch_history(const HistoryArgs& a, const IdT* ids, cudaStream_t st) {
     const int64_t mean = a.offsets ? a.total / a.n_rows : a.columns;     // ids a row, as far as the host knows
     // A row with at least as many ids as there are tokens is counted in shared memory first (8 x 1,048,576 ids of bytes:
-    // 16 us; entered one by one they queue up at ten counters a row: 10,800 us).  A row that is only marked needs 32
+    // 10.8 us; entered one by one they queue up at ten counters a row: 10,800 us).  A row that is only marked needs 32
     // times less to clear and to join.
     const int64_t words = (a.width + 31) / 32, table = a.counts ? a.width : words;
     if (mean >= 1024 && mean >= (a.counts ? table : 4 * table) && table * 4 <= 192 * 1024 && a.n_rows <= (1 << 20)) {
-        int64_t splits = ((int64_t)SMS * 3 + a.n_rows - 1) / a.n_rows;
+        // up to 8 counters a token (8 x 1,048,576 ids of bytes: 10.8 us, 12.4 with 32, which take longer to clear and to join)
+        int log_copies = 0;
+        while (a.counts && log_copies < 3 && (table << (log_copies + 1)) * 4 <= 48 * 1024) ++log_copies;
+        int64_t resident = 220 * 1024 / ((table << log_copies) * 4 + 1024);       // blocks an SM, all of them at once
+        if (resident > 3) resident = 3;
+        int64_t splits = (int64_t)SMS * resident / a.n_rows;
         const int64_t least = table > 1024 ? table : 1024;                // ids a block
         if (splits > mean / least) splits = mean / least;
         if (splits < 1) splits = 1;
-        int log_copies = 0;
-        while (a.counts && log_copies < 5 && (table << (log_copies + 1)) * 4 <= 64 * 1024 && (table << (log_copies + 1)) <= mean / splits) ++log_copies;
+        while (log_copies > 0 && (table << log_copies) > mean / splits) --log_copies;
         const size_t shared = (size_t)(table << log_copies) * 4;
         const unsigned grid = (unsigned)(a.n_rows * splits);
         if (a.counts) {
@@ -283,15 +288,15 @@ int launch_history(const HistoryArgs& a, const IdT* ids, cudaStream_t st) {
         }
         return DNATOK_OK;
     }
-    int group = 1;                                                        // threads a row: about one for four ids
-    while (group < HISTORY_THREADS && group * 4 < mean) group *= 2;
-    int64_t splits = (mean + group * 8 - 1) / (group * 8);
-    const int64_t most = (int64_t)SMS * 2048 / group / a.n_rows;
+    int log_group = 0;                                                    // threads a row: about one for four ids
+    while (1 << log_group < HISTORY_THREADS && 4ll << log_group < mean) ++log_group;
+    int64_t splits = (mean + (8ll << log_group) - 1) / (8ll << log_group);
+    const int64_t most = ((int64_t)SMS * 2048 >> log_group) / a.n_rows;
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
-    const int64_t blocks = (a.n_rows * splits * group + HISTORY_THREADS - 1) / HISTORY_THREADS;
+    const int64_t blocks = ((a.n_rows * splits << log_group) + HISTORY_THREADS - 1) / HISTORY_THREADS;
     if (blocks > INT32_MAX) return abi_fail(DNATOK_ERR_UNSUPPORTED, "too many rows for one call");
-    history_add_kernel<IdT><<<(unsigned)blocks, HISTORY_THREADS, 0, st>>>(a, ids, group, (int)splits);
+    history_add_kernel<IdT><<<(unsigned)blocks, HISTORY_THREADS, 0, st>>>(a, ids, log_group, (int)splits);
     LAUNCH_CHECK("history_add_kernel");
     return DNATOK_OK;
 }
@@ -455,8 +460,9 @@ int launch_allowed(const GrammarTables& t, const int32_t* states, const void* to
     };
     auto marked = [&](auto s, auto n, auto c) { if (t.n_runs * 2 > t.n_groups) run(s, n, c, std::true_type()); else run(s, n, c, std::false_type()); };
     auto placed = [&](auto s, auto n) { if (parts > 1) marked(s, n, std::true_type()); else marked(s, n, std::false_type()); };
-    auto typed = [&](auto s) { if (near) placed(s, std::true_type()); else placed(s, std::false_type()); };
-    if (t.step16) typed(uint16_t()); else typed(uint32_t());
+    if (!t.step16) placed(uint32_t(), std::false_type());              // (such a table is never small)
+    else if (near) placed(uint16_t(), std::true_type());
+    else placed(uint16_t(), std::false_type());
     if (e != cudaSuccess) return abi_fail(DNATOK_ERR_CUDA, "launch of grammar_allowed_kernel: %s", cudaGetErrorString(e));
     LAUNCH_CHECK("grammar_allowed_kernel");
     return DNATOK_OK;

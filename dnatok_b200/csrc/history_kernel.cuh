@@ -4,6 +4,7 @@
 // counts are raised by atomics on whole numbers, so that the order in which they happen does not show.  An id outside
 // the vocabulary is no token, a history row outside the history takes nothing.
 #pragma once
+#include <type_traits>
 #include "common.cuh"
 
 namespace dnatok {
@@ -43,22 +44,22 @@ __device__ __forceinline__ int64_t history_row(const HistoryArgs& a, int64_t row
     return h >= 0 && h < a.history_rows ? h : -1;
 }
 
-// Rows shorter than the vocabulary: `group` threads (a power of two) of one of `splits` parts of a row take its ids in turn
-// and enter them where they belong.  Four ids a thread are under way at a time.
+// Rows shorter than the vocabulary: 2^log_group threads of one of `splits` parts of a row take its ids in turn and enter them
+// where they belong.  Four ids a thread are under way at a time.
 template <typename IdT>
 __global__ void __launch_bounds__(HISTORY_THREADS)
-history_add_kernel(HistoryArgs a, const IdT* __restrict__ ids, int group, int splits) {
+history_add_kernel(HistoryArgs a, const IdT* __restrict__ ids, int log_group, int splits) {
     const int64_t words = (a.width + 31) / 32;
-    const int64_t unit = ((int64_t)blockIdx.x * HISTORY_THREADS + threadIdx.x) / group;
-    const int64_t row = unit / splits;
+    const int64_t unit = ((int64_t)blockIdx.x * HISTORY_THREADS + threadIdx.x) >> log_group;
+    const int64_t row = splits == 1 ? unit : unit / splits;
     if (row >= a.n_rows) return;
     int64_t lo, hi;
     const int64_t h = history_row(a, row, &lo, &hi);
     if (h < 0) return;
     uint32_t* seen = a.seen + h * words;
     int32_t* counts = a.counts ? a.counts + h * a.width : nullptr;
-    const int64_t step = (int64_t)group * splits;
-    for (int64_t i = lo + (unit % splits) * group + (threadIdx.x & (group - 1)); i < hi; i += 4 * step) {
+    const int64_t step = (int64_t)splits << log_group;
+    for (int64_t i = lo + ((unit - row * splits) << log_group) + (threadIdx.x & ((1 << log_group) - 1)); i < hi; i += 4 * step) {
         int64_t id[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) id[k] = i + k * step < hi ? (int64_t)ids[i + k * step] : -1;
@@ -81,6 +82,31 @@ __device__ __forceinline__ void history_part(int64_t& lo, int64_t& hi, int split
     hi = lo + each < end ? lo + each : end;
 }
 
+// f(id) for every id of [lo, hi) that is a token, by the block's threads; eight loads a thread are under way at a time.  (In
+// steps of 2^30 ids, so that the places inside one fit 32 bits.)
+template <typename IdT, typename F>
+__device__ __forceinline__ void history_each(const IdT* __restrict__ ids, int64_t lo, int64_t hi, int width, F f) {
+    using Unsigned = typename std::conditional<sizeof(IdT) == 8, uint64_t, uint32_t>::type;     // below 0: beyond every width
+    constexpr int64_t STEP = 1 << 30;
+    constexpr int EACH = 8;
+    for (; lo < hi; lo += STEP) {
+        const Unsigned* p = reinterpret_cast<const Unsigned*>(ids) + lo;
+        const int n = (int)(hi - lo < STEP ? hi - lo : STEP);
+        int i = threadIdx.x;
+        for (; i + (EACH - 1) * HISTORY_LONG_THREADS < n; i += EACH * HISTORY_LONG_THREADS) {
+            Unsigned id[EACH];
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) id[k] = p[i + k * HISTORY_LONG_THREADS];
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) if (id[k] < (Unsigned)width) f((int)id[k]);
+        }
+        for (; i < n; i += HISTORY_LONG_THREADS) {
+            const Unsigned id = p[i];
+            if (id < (Unsigned)width) f((int)id);
+        }
+    }
+}
+
 // Long rows, counted: a block counts its part of a row in shared memory and then adds what it found.  A long row of few
 // different tokens (bases) would queue up at a handful of counters: there are 2^log_copies of each, one for every 32 / copies
 // lanes of a warp, in banks of their own.
@@ -98,14 +124,7 @@ history_count_kernel(HistoryArgs a, const IdT* __restrict__ ids, int splits, int
     for (int v = threadIdx.x; v < width << log_copies; v += HISTORY_LONG_THREADS) found[v] = 0;
     __syncthreads();
     const int copy = threadIdx.x & (copies - 1);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 8 * HISTORY_LONG_THREADS) {
-        int64_t id[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) id[k] = i + k * HISTORY_LONG_THREADS < hi ? (int64_t)ids[i + k * HISTORY_LONG_THREADS] : -1;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (id[k] >= 0 && id[k] < width) atomicAdd(found + (((int)id[k] << log_copies) | copy), 1);
-    }
+    history_each(ids, lo, hi, width, [&](int id) { atomicAdd(found + ((id << log_copies) | copy), 1); });
     __syncthreads();
     const int words = (width + 31) / 32;
     for (int v = threadIdx.x; v < words * 32; v += HISTORY_LONG_THREADS) {
@@ -132,18 +151,10 @@ history_mark_kernel(HistoryArgs a, const IdT* __restrict__ ids, int splits) {
     const int width = (int)a.width, words = (width + 31) / 32;
     for (int w = threadIdx.x; w < words; w += HISTORY_LONG_THREADS) marked[w] = 0;
     __syncthreads();
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 8 * HISTORY_LONG_THREADS) {
-        int64_t id[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) id[k] = i + k * HISTORY_LONG_THREADS < hi ? (int64_t)ids[i + k * HISTORY_LONG_THREADS] : -1;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (id[k] < 0 || id[k] >= width) continue;
-            uint32_t* word = marked + ((int)id[k] >> 5);
-            const uint32_t bit = 1u << (id[k] & 31);
-            if (!(*reinterpret_cast<volatile uint32_t*>(word) & bit)) atomicOr(word, bit);
-        }
-    }
+    history_each(ids, lo, hi, width, [&](int id) {
+        const uint32_t bit = 1u << (id & 31);
+        if (!(*reinterpret_cast<volatile uint32_t*>(marked + (id >> 5)) & bit)) atomicOr(marked + (id >> 5), bit);
+    });
     __syncthreads();
     for (int w = threadIdx.x; w < words; w += HISTORY_LONG_THREADS)
         if (marked[w]) atomicOr(a.seen + h * words + w, marked[w]);

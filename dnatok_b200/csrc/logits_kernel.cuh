@@ -84,7 +84,6 @@ process_each_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
 // mended afterwards: the warp lists their columns in shared memory and takes 32 of them at a time.
 constexpr int LOGITS_PART = 256;
 constexpr int LOGITS_WARPS = LOGITS_THREADS / 32;
-constexpr int LOGITS_BLOCKS = 4;                   // an SM: 64 registers a thread
 enum { APART, CONTIGUOUS, HALVES };
 
 template <int MAP> __device__ __forceinline__ int tile_column(int lane, int j) {

@@ -323,7 +323,8 @@ size_t dnatok_logits_scratch_bytes(int64_t n_rows, int64_t width);
 /* The gradient of dnatok_process_logits for d_grad (the gradient of its output; the output's type): d_dlogits (the
  * logits' type; NULL: not wanted) and d_dbias (float, [width] where bias_stride is 0, else [n_rows, width] contiguous;
  * NULL: not wanted).  in->bias and in->counts are not read.  A shared bias' gradient is summed in 32 bits in an order
- * that depends on the sizes only.  d_dlogits may be d_grad itself where type and stride are the same. */
+ * that depends on the sizes only.  d_dlogits may be d_grad itself where type and stride are the same; it may
+ * not be the logits. */
 int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, int32_t grad_dtype, int64_t grad_stride,
                                    void* d_dlogits, int64_t dlogits_stride, float* d_dbias, void* d_scratch,
                                    size_t scratch_bytes, dnatok_stream stream);

@@ -39,7 +39,7 @@ def test_c_abi_refuses_bad_outputs():
     half = logits_struct(dtype=2)
     assert L.dnatok_process_logits(ctypes.byref(half), 4096, 0, 40, None) == INVALID         # in place as another type
     for args in [(None, 0, 40, 12288, 40, None), (8192, 1, 40, 12288, 40, None), (8192, 0, -1, 12288, 40, None), (8192, 0, 40, 12288, 39, None),
-                 (8193, 0, 40, 12288, 40, None), (8192, 0, 40, 12288, 40, 6), (8192, 0, 41, 8192, 40, None)]:
+                 (8193, 0, 40, 12288, 40, None), (8192, 0, 40, 12288, 40, 6), (8192, 0, 41, 8192, 40, None), (8192, 0, 40, 4096, 40, None)]:
         assert L.dnatok_process_logits_backward(ctypes.byref(a), *args, None, 0, None) == INVALID
     assert L.dnatok_process_logits(None, 8192, 0, 40, None) == INVALID
 

@@ -98,6 +98,54 @@ def test_the_tokenizers_vocabularies(name):
         tok.grammar(automaton, width=tok.vocab_size - 1)
 
 
+@pytest.mark.parametrize("n", [1, 60, 300, 700])
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("vocabulary", ["kmer", "words"])
+def test_vocabularies_and_batches(vocabulary, large, n):
+    """Every way of dividing a call: a row over several blocks or one, small and large tables, tokens whose ids follow one
+    another in the order of their text (at any place of a word) and others."""
+    import itertools
+    rng = np.random.default_rng([n, large])
+    tokens = [b""] * 7 + [bytes(t) for t in itertools.product(b"ACGT", repeat=6)] if vocabulary == "kmer" else random_tokens(rng, 9000, 12, b"ACGT")
+    if large:
+        nxt = np.full((3001, 5), -1)
+        for c in range(4):
+            keep = rng.random(3000) < 0.6
+            nxt[:3000][keep, c] = np.arange(1, 3001)[keep]
+        nxt[3000, :4] = 3000                                       # after the pattern, anything
+        automaton = Automaton(nxt, np.arange(3001) == 3000)
+    else:
+        automaton = Automaton.avoiding(["GAATTC", "TTT", "CCWGG", "ACGT"])
+    states = some_states(rng, automaton, n)
+    states[-1] = automaton.n_states - 1
+    check(automaton, tokens, 3, states, rng.integers(0, len(tokens), n))
+
+
+def test_a_grammar_is_closed_while_a_graph_is_captured():
+    a = Automaton.avoiding(["ACG"])
+    tokens = [b"A", b"AC", b"ACG", b"T"]
+    keep, gone = Grammar(a, tokens), Grammar(a, tokens)
+    states = torch.zeros(3, dtype=torch.int32, device="cuda")
+    want = keep.allowed(states)
+    gone.allowed(states)
+    torch.cuda.synchronize()
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(want)
+    with torch.cuda.graph(graph):
+        keep.allowed(states, out=out)
+        gone.close()
+    graph.replay()
+    assert torch.equal(out, want)
+    fresh = Grammar(a, tokens)
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other):
+        keep.allowed(states, out=out)
+        with pytest.raises(RuntimeError, match="outside of stream capture"):
+            fresh.allowed(states, out=out)
+    out.zero_()
+    other.replay()
+    assert torch.equal(out, want)
+
+
 def test_long_tokens_and_a_long_pattern():
     """Tokens of hundreds of bases among short ones; a pattern of thousands of positions."""
     rng = np.random.default_rng(6)

@@ -181,6 +181,68 @@ def test_words_behind_the_last_token_are_not_looked_at():
     assert torch.equal(process_logits(d["x"], allowed=ok, **kw), y)
 
 
+# Calls beyond what a thread a logit serves: tiles of one and of two parts, vectors of 16 bits, halves beside 32 bits, columns
+# apart; tiles and pieces that end anywhere; more rows than a grid has blocks for.
+LARGE = [(40, 8192, 0, 0), (40, 8192, 1, 7), (40, 8192, 8, 8), (400, 4096, 0, 0), (400, 4100, 0, 0), (700, 1001, 0, 0), (90, 4106, 0, 0),
+         (61000, 5, 0, 0), (3, 120007, 0, 0), (500, 616, 0, 0), (12, 32000, 0, 4), (530001, 1, 0, 0)]
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("n,width,shift,pad", LARGE)
+def test_large_calls(n, width, shift, pad, dtype):
+    d = make(n, width, dtype, seed=13, shift=shift, pad=pad, history_rows=n if n < 1000 else 50)
+    seen, counts, rows = d["seen"], d["counts"], None
+    if n >= 1000:
+        target = np.random.default_rng(1).integers(-5, 55, n)
+        inside = (target >= 0) & (target < 50)
+        at = np.where(inside, target, 0)
+        seen, counts = seen[at] & inside[:, None], counts[at] * inside[:, None]
+        rows = torch.from_numpy(target).cuda()
+    x = R.host(d["x"])
+    pen = dict(history=d["h"], rows=rows, repetition=cuda(d["r"]), frequency=cuda(d["f"]), presence=cuda(d["p"]))
+    ref = dict(seen=seen, counts=counts, r=d["r"], f=d["f"], p=d["p"])
+    for out_dtype in {dtype, torch.float32}:
+        for kw, more in [(dict(bias=cuda(d["bias"]), allowed=words(d["ok"]), **pen), dict(bias=d["bias"], ok=d["ok"], **ref)),
+                         (dict(bias=cuda(d["bias"][0]), allowed=words(d["ok"][:1])), dict(bias=d["bias"][:1], ok=np.broadcast_to(d["ok"][:1], (n, width)))),
+                         (pen, ref)]:
+            want, bound = R.logits(x, **more)
+            y = process_logits(d["x"], out_dtype=out_dtype, **kw)
+            R.close(y, want, bound, out_dtype)
+            if out_dtype == dtype:
+                z = d["x"].clone() if shift == 0 else d["x"]
+                assert torch.equal(process_logits(z, out=z, **kw), y)
+                if z is d["x"]:
+                    d["x"].copy_(torch.from_numpy(x).to(dtype))
+    g = cuda(d["grad"]).to(dtype)
+    for bias in (cuda(d["bias"]), cuda(d["bias"][0]), None):
+        dx, db = process_logits_backward(g, d["x"], bias=bias, allowed=words(d["ok"]), **pen)
+        want, each = R.gradients(x, R.host(g), seen, d["r"], d["ok"])
+        R.close(dx, want, np.abs(want) * 2 * R.U32, dtype)
+        if bias is None:
+            assert db is None
+        elif bias.dim() == 2:
+            R.close(db, each, 0.0, torch.float32)
+        else:
+            R.close(db, each.sum(0), 1.01 * n * R.U32 * np.abs(each).sum(0), torch.float32)
+    dx, _ = process_logits_backward(g, d["x"])                     # nothing but the identity
+    assert torch.equal(dx, g)
+
+
+@pytest.mark.parametrize("width", [512, 4106, 32000])
+def test_rows_that_have_seen_everything(width):
+    n = 3 * 10 ** 5 // width + 30
+    d = make(n, width, torch.bfloat16, seed=14)
+    d["h"].seen.fill_(-1)
+    d["h"].counts.fill_(7)
+    full = np.ones((n, width), dtype=bool)
+    kw = dict(history=d["h"], repetition=cuda(d["r"]), frequency=cuda(d["f"]), presence=0.125)
+    want, bound = R.logits(R.host(d["x"]), full, full * 7, d["r"], d["f"], 0.125)
+    R.close(process_logits(d["x"], **kw), want, bound, torch.bfloat16)
+    g = cuda(d["grad"]).to(torch.bfloat16)
+    want, _ = R.gradients(R.host(d["x"]), R.host(g), full, d["r"])
+    R.close(process_logits_backward(g, d["x"], **kw)[0], want, np.abs(want) * 2 * R.U32, torch.bfloat16)
+
+
 # --------------------------------------------------------------------------- gradients
 
 @pytest.mark.parametrize("dtype", R.TYPES)
