@@ -311,15 +311,17 @@ process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride)
     }
 }
 
-// The gradients of the logits at a row's hits, over those of its other allowed tokens.
-template <int PARTS, typename T, typename G>
-__device__ __forceinline__ void mend_gradient(const LogitsArgs& a, int row, uint32_t hits, uint16_t* list, const T* x_row, const G* g_row, T* d_row, int lane) {
-    if (!__any_sync(0xffffffffu, hits)) return;
-    const int n_hits = list_hits<PARTS>(hits, list, lane);           // (its barrier also puts the stores in order)
+// The gradients of the logits at a row's hits, over those of its other allowed tokens.  x: the logit of this lane's first hit,
+// fetched ahead of time.
+template <typename T, typename G>
+__device__ __forceinline__ void mend_gradient(const LogitsArgs& a, int row, int n_hits, const uint16_t* list, T x, const T* x_row, const G* g_row, T* d_row, int lane) {
+    __syncwarp();                                             // the order of the stores
     const Penalty pen = penalty_of(of_row(a.d_repetition, a.repetition, row));
     for (int i = lane; i < n_hits; i += 32) {
         const int v = list[i];
-        d_row[v] = from_float<T>(penalise(pen, as_float(x_row[v]), as_float(g_row[v])));
+        const T now = x;
+        if (i + 32 < n_hits) x = x_row[list[i + 32]];
+        d_row[v] = from_float<T>(penalise(pen, as_float(now), as_float(g_row[v])));
     }
     __syncwarp();
 }
@@ -342,6 +344,13 @@ logits_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_t gra
         }
         const uint32_t ok = a.allowed ? tile_word<PARTS>(a.allowed + (row * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
         const uint32_t hits = SEEN ? tile_hits<PARTS>(a, history_of(a, row), ok, base, left, lane) : 0;
+        const T* x_row = logits + (row * a.stride + base);
+        int n_hits = 0;
+        T x = {};
+        if (SEEN && __any_sync(0xffffffffu, hits)) {
+            n_hits = list_hits<PARTS>(hits, listed[threadIdx.x >> 5], lane);
+            if (lane < n_hits) x = x_row[listed[threadIdx.x >> 5][lane]];
+        }
         T* d_row = dlogits ? dlogits + (row * dlogits_stride + base) : nullptr;
 #pragma unroll
         for (int u = 0; u < PARTS; ++u) {
@@ -352,7 +361,7 @@ logits_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_t gra
             if (dbias) store_tile<MAP>(dbias + ((int64_t)row * a.width + base + u * LOGITS_PART), all, lane, g);
             if (d_row) store_tile<MAP>(d_row + u * LOGITS_PART, all, lane, g);
         }
-        if (SEEN) mend_gradient<PARTS>(a, row, hits, listed[threadIdx.x >> 5], logits + (row * a.stride + base), g_row, d_row, lane);
+        if (SEEN && n_hits) mend_gradient(a, row, n_hits, listed[threadIdx.x >> 5], x, x_row, g_row, d_row, lane);
     }
 }
 
@@ -366,7 +375,7 @@ logits_bias_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_
                             float* sums, int rows_per_block) {
     constexpr int R = 2;                                      // rows under way at a time
     __shared__ float part[LOGITS_WARPS][LOGITS_PART * PARTS];
-    __shared__ uint16_t listed[SEEN ? LOGITS_WARPS : 1][LOGITS_PART * PARTS];
+    __shared__ uint16_t listed[SEEN ? LOGITS_WARPS : 1][R][LOGITS_PART * PARTS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int base = blockIdx.x * LOGITS_PART * PARTS, left = a.width - base;
     const int first = blockIdx.y * rows_per_block, last = a.n_rows - first < rows_per_block ? a.n_rows : first + rows_per_block;
@@ -386,7 +395,17 @@ logits_bias_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_
                 for (int u = 0; u < PARTS; ++u)
                     load_tile<MAP>(grad + (i * grad_stride + base + u * LOGITS_PART), tile_all<MAP>(left - u * LOGITS_PART, lane), lane, raw[k][u]);
                 ok[k] = a.allowed ? tile_word<PARTS>(a.allowed + (i * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
-                if (SEEN && dlogits) hits[k] = tile_hits<PARTS>(a, history_of(a, i), ok[k], base, left, lane);
+                if (SEEN) hits[k] = tile_hits<PARTS>(a, history_of(a, i), ok[k], base, left, lane);
+            }
+        }
+        int n_hits[R] = {};
+        T x[R] = {};
+        if (SEEN) {
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                if (!__any_sync(0xffffffffu, hits[k])) continue;
+                n_hits[k] = list_hits<PARTS>(hits[k], listed[warp][k], lane);
+                if (lane < n_hits[k]) x[k] = logits[(row + k * LOGITS_WARPS) * a.stride + base + listed[warp][k][lane]];
             }
         }
 #pragma unroll
@@ -405,7 +424,8 @@ logits_bias_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_
                 }
                 if (d_row) store_tile<MAP>(d_row + u * LOGITS_PART, tile_all<MAP>(left - u * LOGITS_PART, lane), lane, g);
             }
-            if (SEEN) mend_gradient<PARTS>(a, i, hits[k], listed[warp], logits + (i * a.stride + base), grad + (i * grad_stride + base), d_row, lane);
+            if (SEEN && n_hits[k])
+                mend_gradient(a, i, n_hits[k], listed[warp][k], x[k], logits + (i * a.stride + base), grad + (i * grad_stride + base), d_row, lane);
         }
     }
 #pragma unroll

@@ -82,7 +82,7 @@ def test_the_tokenizers_vocabularies(name):
     tok = B200Tokenizer(H.spec(name))
     text = token_bytes(tok.spec)
     rng = np.random.default_rng(3)
-    for automaton in (Automaton.avoiding(["GAATTC", "CCWGG"], reverse_complement=True), Automaton.from_pattern("ATG(NNN){0,40}TAA(R|Y){0,30}")):
+    for automaton in (Automaton.avoiding(["GAATTC", "CCWGG"], reverse_complement=True), Automaton.from_pattern("ATG(NNN){0,40}TAA(R|Y){0,3}")):
         g = tok.grammar(automaton)
         states = some_states(rng, automaton, 12)
         end = tok.sep_token_id
