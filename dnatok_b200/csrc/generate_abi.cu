@@ -400,7 +400,11 @@ int grammar_tables(dnatok_grammar* g, cudaStream_t stream, GrammarTables* out) {
         t.super_steps = g->super_steps; t.prefix_steps = g->prefix_steps;
         t.width = g->width; t.end_id = g->end_id;
         d.memory = undo.memory;
-        it = g->dev.emplace(dev, d).first;
+        try {
+            it = g->dev.emplace(dev, d).first;
+        } catch (const std::bad_alloc&) {
+            return abi_fail(DNATOK_ERR_INVALID, "out of memory");
+        }
         undo.memory = nullptr;
     }
     *out = it->second.tables;
@@ -417,7 +421,7 @@ int check_states(const dnatok_grammar* g, const void* states, int64_t n_rows) {
 int launch_allowed(const GrammarTables& t, const int32_t* states, const void* tokens, int token_bits, int32_t* states_out, int64_t n_rows,
                    uint32_t* allowed, cudaStream_t st) {
     const int64_t words = (t.width + 31) / 32;
-    // The sorted groups need a row's words in shared memory; vocabularies beyond 262,144 tokens and automata with more than
+    // The groups need a row's words in shared memory, 32 KB beside a small table; vocabularies beyond 262,144 tokens and automata with more than
     // 15 classes go token by token.
     if (!t.text || words > 8192 || n_rows > INT32_MAX / 8) {
         if (tokens) {

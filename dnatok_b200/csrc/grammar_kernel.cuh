@@ -8,9 +8,15 @@
 // prefix, and 32 groups share the beginning of their prefixes.  A row walks those beginnings first, a lane each, then the
 // prefixes of the groups behind the ones that live, a lane a group, and then, a warp a group, only the rest of the tokens
 // whose prefix lives: automata that allow little leave most tokens after a few steps for 1,024 of them, and one that allows
-// nearly all walks the shared bases once.  (The order trades the length of the prefixes, which is what a row that allows
-// little lives by, against the steps behind them, which are those of a group's longest token: with 32,000 random tokens 9
-// in one order of all texts, 3 within each length, 4 this way.)
+// nearly all walks the shared bases once.  (The order trades the length of the prefixes,
+// which is what a row that allows little lives by, against the steps behind them, those of a group's longest token: with
+// 32,000 random tokens 3.3 bases and 4.8 steps this way, 3.7 and 6.4 in one order of all texts.  Groups cut at the nodes of
+// the texts' trie share 4.7 bases and halve a typical row of a pattern, 22 -> 10 us for 1,024 of them, but there are 1.6
+// times as many: rows that allow nearly all, which the others wait for, go from 95 to 165 us.)
+//
+// What bounds it: instructions, about 85 a group and warp with its share of everything (1,024 rows of a 2,000-position
+// pattern over 32,000 tokens: 9.2 M, 33 us, of which the last third is a few rows that allow most tokens), and for few rows
+// the latency of the dependent loads (one row 5 to 6 us).  The bytes are nothing: 4 MB of masks.
 #pragma once
 #include <cooperative_groups.h>
 #include <type_traits>
@@ -109,12 +115,13 @@ grammar_any_kernel(GrammarTables t, const int32_t* __restrict__ states, int64_t 
 
 // A cluster of `parts` blocks takes a row.  Its warps share the sets of 32 groups that live (`split` warps a set: each takes
 // every split-th of the groups); the tokens that live set their bits in the block's shared memory, and each block joins and
-// writes its share of the words.  All counts are powers of two.  With `tokens` the row's state is advanced
-// first (by every thread for itself) and written by the cluster's first.  NEAR: the table is small and copied to shared
-// memory, so that a walk's steps do not each wait for the L2 the first time (it is worth its copy up to 16 KB).
+// writes its share of the words.  All counts are powers of two.  With `tokens` the row's state is advanced first (by every
+// thread for itself: a warp that does it for the others keeps them waiting, 31 -> 39 us) and written by the cluster's first.
+// NEAR: the table is small and copied to shared memory, so that a walk's steps do not each wait for the L2 the first time.
+// RUNS: many groups' ids follow one another, as those of k-mers do; their bits are set as one word, since 32 lanes would
+// queue up at it (1,024 rows of 6-mers: 18 us, 22 without).
 constexpr int GRAMMAR_NEAR_BYTES = 16 * 1024;
-
-constexpr int GRAMMAR_MOST = 512;                              // threads a block
+constexpr int GRAMMAR_MOST = 512;                             // threads a block; 40 registers: 3 blocks an SM
 
 template <typename S, bool NEAR, bool CLUSTER, bool RUNS>
 __global__ void __launch_bounds__(GRAMMAR_MOST, 3)

@@ -228,6 +228,28 @@ def test_large_calls(n, width, shift, pad, dtype):
     assert torch.equal(dx, g)
 
 
+def test_offsets_beyond_32_bits():
+    """70,001 x 32,000 logits and a history as large: the last rows as in a call of their own."""
+    n, width, last = 70001, 32000, 3
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty((n, width), dtype=torch.bfloat16, device="cuda").normal_(0, 3, generator=g)
+    h = TokenHistory(n, width)
+    h.append(torch.randint(0, width, (n,), generator=g, device="cuda"))
+    h.append(torch.randint(0, width, (n,), generator=g, device="cuda"))
+    small = TokenHistory(last, width)
+    small.seen.copy_(h.seen[-last:])
+    small.counts.copy_(h.counts[-last:])
+    assert small.counts.sum() == 2 * last and h.counts[0].sum() == 2
+    bias = torch.randn(width, generator=g, device="cuda")
+    ok = torch.randint(-2 ** 31, 2 ** 31, (n, width // 32), generator=g, device="cuda").int()
+    kw = dict(repetition=1.5, frequency=0.25, presence=0.5, bias=bias)
+    y = process_logits(x, history=h, allowed=ok, **kw)
+    assert torch.equal(y[-last:], process_logits(x[-last:], history=small, allowed=ok[-last:], **kw))
+    dx, db = process_logits_backward(y.nan_to_num_(0, 0, 0), x, history=h, allowed=ok, **kw)
+    want, _ = process_logits_backward(y[-last:], x[-last:], history=small, allowed=ok[-last:], **kw)
+    assert torch.equal(dx[-last:], want) and torch.isfinite(db).all()
+
+
 @pytest.mark.parametrize("width", [512, 4106, 32000])
 def test_rows_that_have_seen_everything(width):
     n = 3 * 10 ** 5 // width + 30
