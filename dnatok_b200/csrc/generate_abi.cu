@@ -119,13 +119,14 @@ dim3 logits_grid(int64_t n_rows, int64_t width, int parts) {
 }
 
 // With a shared bias' gradient a block goes through several groups of rows, as many as leave at most 12 blocks an SM (three
-// whole rounds of 4, four of 3): their partial sums are few beside what they read.
+// whole rounds of 4, four of 3): their partial sums are few beside what they read.  Up to 32 rows one block does them all,
+// four a warp: that takes less than a second launch to join two.
 dim3 bias_grid(int64_t n_rows, int64_t width, int parts) {
     const int64_t tiles = tiles_of(width, parts);
     int64_t groups = (int64_t)SMS * 12 / tiles;
     const int64_t most = (n_rows + LOGITS_WARPS - 1) / LOGITS_WARPS;
     if (groups > most) groups = most;
-    if (groups < 1) groups = 1;
+    if (groups < 1 || n_rows <= 32) groups = 1;
     const int64_t rows = rows_per_block(n_rows, groups);
     return dim3((unsigned)tiles, (unsigned)((n_rows + rows - 1) / rows));
 }

@@ -39,6 +39,7 @@ _TYPES = {torch.float32: _cabi.F32, torch.float16: _cabi.F16, torch.bfloat16: _c
 _BITS = {torch.int32: 32, torch.int64: 64}
 
 Number = Union[float, int, torch.Tensor]
+_LEAST, _MOST = 2.0 ** -126, 2.0 ** 126              # a repetition penalty whose reciprocal is a normal number too
 
 
 # The current stream of a device as a number (the public call builds a Stream object on the way: 2 us instead of 0.1).
@@ -309,9 +310,12 @@ class Grammar:
 
 # --------------------------------------------------------------------------- logits
 
-def _rows_of(t: torch.Tensor, what: str) -> None:
-    if t.dim() != 2 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
+def _rows_of(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
+    """(rows, columns, elements from row to row)."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < 1 or (shape[1] > 1 and strides[1] != 1):
         raise ValueError("%s must be a tensor [n, width] whose rows are contiguous" % what)
+    return shape[0], shape[1], strides[0]
 
 
 def _penalty(name: str, v, n: int, dev: int):
@@ -325,8 +329,8 @@ def _penalty(name: str, v, n: int, dev: int):
             raise ValueError("%s has no gradient" % name)
         return neutral, v.data_ptr(), True
     v = float(v)
-    if name == "repetition":
-        if not 2.0 ** -126 <= v <= 2.0 ** 126:
+    if neutral:
+        if not _LEAST <= v <= _MOST:
             raise ValueError("repetition must be positive and finite (2^-126 to 2^126)")
     elif v - v != 0.0:
         raise ValueError("%s must be finite" % name)
@@ -356,13 +360,12 @@ def _row_array(t, what: str, dtype, n: int, columns: int, dev: int) -> Tuple[int
 def _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed):
     """(the C arguments, the number of the GPU)."""
     dev = _device_of(logits, "logits")
-    _rows_of(logits, "logits")
+    n, width, stride = _rows_of(logits, "logits")
     dtype = _TYPES.get(logits.dtype)
     if dtype is None:
         raise ValueError("logits must be float32, float16 or bfloat16")
-    n, width = logits.shape
     a = _cabi.Logits()
-    a.logits, a.dtype, a.n_rows, a.width, a.stride = logits.data_ptr(), dtype, n, width, logits.stride(0)
+    a.logits, a.dtype, a.n_rows, a.width, a.stride = logits.data_ptr(), dtype, n, width, stride
     a.repetition, a.d_repetition, once = _penalty("repetition", repetition, n, dev)
     a.frequency, a.d_frequency, often = _penalty("frequency", frequency, n, dev)
     a.presence, a.d_presence, also = _penalty("presence", presence, n, dev)
@@ -481,7 +484,7 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
 
     All of it is computed in 32 bits and rounded once.  Differentiable in ``logits`` and ``bias``; the history and the mask
     must then stay as they are until the backward pass (autograd refuses it otherwise)."""
-    if torch.is_grad_enabled() and (getattr(logits, "requires_grad", False) or getattr(bias, "requires_grad", False)):
+    if (getattr(logits, "requires_grad", False) or (bias is not None and getattr(bias, "requires_grad", False))) and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out= has no gradient; leave it out or call under torch.no_grad()")
         return _Process.apply(logits, bias, history, rows, repetition, frequency, presence, allowed, out_dtype)

@@ -400,6 +400,25 @@ def test_another_stream_and_a_captured_graph():
     assert alive.requires_grad
 
 
+def test_forward_and_gradient_in_one_captured_graph():
+    n, width = 20, 1000
+    d = make(n, width, torch.float32, seed=15)
+    kw = dict(history=d["h"], repetition=cuda(d["r"]), frequency=0.5, presence=0.5, allowed=words(d["ok"]))
+    x, b, g = d["x"].clone().requires_grad_(), cuda(d["bias"][0]).requires_grad_(), cuda(d["grad"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = process_logits(x, bias=b, **kw)
+        dx, db = torch.autograd.grad(y, (x, b), g)
+    for k in range(2):
+        with torch.no_grad():
+            x.add_(k)
+        dx.zero_()
+        graph.replay()
+        want, each = R.gradients(R.host(x), d["grad"], d["seen"], d["r"], d["ok"])
+        R.close(dx, want, np.abs(want) * 2 * R.U32, torch.float32)
+        R.close(db, each.sum(0), 1.01 * n * R.U32 * np.abs(each).sum(0), torch.float32)
+
+
 def test_refusals():
     d = make(3, 64, torch.float32, seed=12)
     x, h = d["x"], d["h"]
