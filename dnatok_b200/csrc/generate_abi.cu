@@ -436,15 +436,14 @@ int launch_allowed(const GrammarTables& t, const int32_t* states, const void* to
         return DNATOK_OK;
     }
     // Few rows: up to 8 blocks a row, as long as all are on the GPU at once (3 an SM) and each has 128 groups.  A warp for
-    // every 4 groups, up to 16; 8 where rows fill the GPU by themselves.  (1,024 rows of a pattern over 32,000 tokens: 31 us
-    // with 8, 54 with 4, because the rows differ and one that may go on with anything holds up the rest; 148 such rows: 20 us
-    // in 296 blocks, 25 in 592, which are two rounds.)
+    // every 4 groups, up to 16: rows differ, and one that may go on with anything holds up the others (1,024 rows of a pattern
+    // over 32,000 tokens: 29 us, 35 with 8 warps, 47 in clusters of 2 blocks; 148 rows that all may: 20 us in 296 blocks, 25 in
+    // 592, which are two rounds).
     const int64_t room = (int64_t)SMS * 3;
     int parts = 1;
     while (parts < 8 && n_rows * parts * 2 <= room && t.n_groups > parts * 128) parts *= 2;
     int warps = 1;
-    const int most = n_rows > room ? 8 : GRAMMAR_MOST / 32;
-    while (warps < most && warps * 4 * parts < t.n_groups) warps *= 2;
+    while (warps < GRAMMAR_MOST / 32 && warps * 4 * parts < t.n_groups) warps *= 2;
     int split = 1;                                            // warps a set of 32 groups
     while (split < 32 && split < warps * parts && t.n_super * split < warps * parts) split *= 2;
     const size_t table = (((size_t)(t.n_states + 1) << t.log_pitch) * (t.step16 ? 2 : 4) + 15) / 16 * 16;

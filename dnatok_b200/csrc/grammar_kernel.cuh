@@ -15,7 +15,7 @@
 // times as many: rows that allow nearly all, which the others wait for, go from 95 to 165 us.)
 //
 // What bounds it: instructions, about 85 a group and warp with its share of everything (1,024 rows of a 2,000-position
-// pattern over 32,000 tokens: 9.2 M, 33 us, of which the last third is a few rows that allow most tokens), and for few rows
+// pattern over 32,000 tokens: 11 M, 29 us, of which the last third is a few rows that allow most tokens), and for few rows
 // the latency of the dependent loads (one row 5 to 6 us).  The bytes are nothing: 4 MB of masks.
 #pragma once
 #include <cooperative_groups.h>
@@ -119,7 +119,7 @@ grammar_any_kernel(GrammarTables t, const int32_t* __restrict__ states, int64_t 
 // thread for itself: a warp that does it for the others keeps them waiting, 31 -> 39 us) and written by the cluster's first.
 // NEAR: the table is small and copied to shared memory, so that a walk's steps do not each wait for the L2 the first time.
 // RUNS: many groups' ids follow one another, as those of k-mers do; their bits are set as one word, since 32 lanes would
-// queue up at it (1,024 rows of 6-mers: 18 us, 22 without).
+// queue up at it (1,024 rows of 4,106 tokens: 18 us, 22 without).
 constexpr int GRAMMAR_NEAR_BYTES = 16 * 1024;
 constexpr int GRAMMAR_MOST = 512;                             // threads a block; 40 registers: 3 blocks an SM
 

@@ -332,8 +332,8 @@ def _penalty(name: str, v, n: int, dev: int):
     if neutral:
         if not _LEAST <= v <= _MOST:
             raise ValueError("repetition must be positive and finite (2^-126 to 2^126)")
-    elif v - v != 0.0:
-        raise ValueError("%s must be finite" % name)
+    elif not abs(v) <= 3.4028234e38:
+        raise ValueError("%s must be a finite float32 number" % name)
     return v, None, v != neutral
 
 

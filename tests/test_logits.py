@@ -427,7 +427,7 @@ def test_refusals():
     plain = TokenHistory(3, 64, counts=False)
     for kw in [dict(repetition=1.5), dict(frequency=0.5), dict(rows=torch.zeros(3, dtype=torch.int32, device="cuda")), dict(history=other, repetition=1.5),
                dict(history=TokenHistory(4, 64), repetition=1.5), dict(history=plain, frequency=0.5), dict(history=h, repetition=0.0),
-               dict(history=h, repetition=math.inf), dict(history=h, presence=math.nan), dict(history=h, repetition=torch.ones(2, device="cuda")),
+               dict(history=h, repetition=math.inf), dict(history=h, presence=math.nan), dict(history=h, frequency=1e300), dict(history=h, repetition=1e-60), dict(history=h, repetition=torch.ones(2, device="cuda")),
                dict(history=h, repetition=torch.ones(3, device="cuda", dtype=torch.float64)), dict(history=h, repetition=torch.ones(3)),
                dict(history=h, repetition=torch.ones(3, device="cuda", requires_grad=True)), dict(history=h, repetition=torch.ones(6, device="cuda")[::2]),
                dict(history=h, rows=torch.zeros(2, dtype=torch.int32, device="cuda"), repetition=1.5),
