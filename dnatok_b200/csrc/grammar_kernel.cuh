@@ -232,7 +232,8 @@ grammar_allowed_kernel(GrammarTables t, const int32_t* __restrict__ states, cons
                     }
                 };
                 while (__popc(alive) >= TOGETHER) walk(std::integral_constant<int, TOGETHER>());
-                while (alive) walk(std::integral_constant<int, 1>());
+                while (__popc(alive) >= 2) walk(std::integral_constant<int, 2>());
+                if (alive) walk(std::integral_constant<int, 1>());
                 while (slow) {                                    // groups with a longer token: from the row's state, code by code
                     const int k = __ffs(slow) - 1;
                     slow &= slow - 1;
