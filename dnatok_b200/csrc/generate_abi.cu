@@ -179,8 +179,13 @@ int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtyp
                 return;
             }
             with_variant<sizeof(T), sizeof(O)>(vector, a.width, a.seen != nullptr, parts, [&](auto m, auto seen, auto n) {
-                process_logits_kernel<T, O, decltype(m)::value, decltype(seen)::value, decltype(n)::value><<<grid, LOGITS_THREADS, 0, st>>>(
-                    a, (const T*)in->logits, (O*)d_out, out_stride);
+                constexpr int MAP = decltype(m)::value, PARTS = decltype(n)::value;
+                if constexpr (!decltype(seen)::value)
+                    process_logits_kernel<T, O, MAP, NO_HISTORY, PARTS><<<grid, LOGITS_THREADS, 0, st>>>(a, (const T*)in->logits, (O*)d_out, out_stride);
+                else if (a.counts)
+                    process_logits_kernel<T, O, MAP, COUNTED, PARTS><<<grid, LOGITS_THREADS, 0, st>>>(a, (const T*)in->logits, (O*)d_out, out_stride);
+                else
+                    process_logits_kernel<T, O, MAP, SEEN_ONLY, PARTS><<<grid, LOGITS_THREADS, 0, st>>>(a, (const T*)in->logits, (O*)d_out, out_stride);
             });
         };
         if (out_dtype == in->dtype) typed(t); else typed((float*)nullptr);

@@ -79,17 +79,19 @@ process_each_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
 //   HALVES      4 and 4 at a distance of 128, where a 32-bit array is among them: its two accesses fill whole sectors
 //   APART       32 apart, at any alignment (a vocabulary of 4,106 tokens in 16 bits, a view that begins anywhere)
 //
-// All columns get bias and mask on this way.  The tokens that a row has seen are few among many, as a rule; penalising 8
-// columns a lane for one of them took more instructions than all the rest together.  So the hits (seen and allowed) are
-// mended afterwards: the warp lists their columns in shared memory and takes 32 of them at a time.
+// All columns get bias, mask and repetition penalty on this way.  Where counts matter too, the hits (seen and allowed) are
+// mended afterwards: they are few among many, as a rule, and fetching and subtracting counts for 8 columns a lane took more
+// instructions than all the rest together.  The warp lists the hits' columns in shared memory and takes 32 at a time.  (The
+// repetition penalty alone, 333 x 32,000 fp16: 12.4 us among all columns, 14.4 by the list.)
 //
 // What bounds it: instructions and memory about alike.  2,048 x 32,000 bf16 to float, a quarter allowed, 5 % seen: 94 us, issue
 // slots 73 % busy, 444 MB = 4.7 TB/s (the counts of scattered tokens cost 64 bytes each from DRAM); 4,096 x 32,000 bf16 with
-// nine tenths allowed: 176 us, 5.3 TB/s; 333 x 32,000 fp16 with the repetition penalty alone 14.4 us, 3 TB/s, instructions
-// (about 100 of 210 per 256 columns and warp are the hits).
+// nine tenths allowed: 176 us, 5.3 TB/s; 333 x 32,000 fp16 with the repetition penalty alone 12.4 us, 3.5 TB/s, of
+// which the launch and the first loads are about 4.
 constexpr int LOGITS_PART = 256;
 constexpr int LOGITS_WARPS = LOGITS_THREADS / 32;
 enum { APART, CONTIGUOUS, HALVES };
+enum { NO_HISTORY, SEEN_ONLY, COUNTED };           // what the penalties need
 
 template <int MAP> __device__ __forceinline__ int tile_column(int lane, int j) {
     return MAP == CONTIGUOUS ? lane * 8 + j : MAP == HALVES ? (j >> 2) * 128 + lane * 4 + (j & 3) : j * 32 + lane;
@@ -206,13 +208,26 @@ __device__ __forceinline__ float penalise(const Penalty& q, float x, float by) {
 template <int PARTS> __device__ __forceinline__ int hit_shift(int lane) { return lane / (8 * PARTS) * (8 * PARTS); }
 template <int PARTS> __device__ __forceinline__ int hit_column(int lane) { return (lane & (8 * PARTS - 1)) * 32 + hit_shift<PARTS>(lane); }
 
+// The words of the tile's hits: what row h of the history has seen among `ok`.
 template <int PARTS>
-__device__ __forceinline__ uint32_t tile_hits(const LogitsArgs& a, int32_t h, uint32_t ok, int base, int left, int lane) {
-    if (h < 0) return 0;
+__device__ __forceinline__ uint32_t hit_word(const LogitsArgs& a, int32_t h, uint32_t ok, int base, int left, int lane) {
+    return h < 0 ? 0 : tile_word<PARTS>(a.seen + ((int64_t)h * ((a.width + 31) >> 5) + (base >> 5)), left, lane) & ok;
+}
+
+// The hits that this lane lists.  (Bits behind the last column are no tokens.)
+template <int PARTS> __device__ __forceinline__ uint32_t lane_hits(uint32_t word, int left, int lane) {
     constexpr int BITS = 8 * PARTS;
-    const uint32_t word = tile_word<PARTS>(a.seen + ((int64_t)h * ((a.width + 31) >> 5) + (base >> 5)), left, lane) & ok;
-    const int behind = left - hit_column<PARTS>(lane);        // (bits behind the last column are no tokens)
+    const int behind = left - hit_column<PARTS>(lane);
     return word >> hit_shift<PARTS>(lane) & ((1u << (behind >= BITS ? BITS : behind > 0 ? behind : 0)) - 1);
+}
+
+// by[j] times the penalty of x[j] where `hit` has a bit.
+__device__ __forceinline__ void penalise_hits(const Penalty& q, uint32_t hit, const float (&x)[8], float (&by)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float z = penalise(q, x[j], by[j]);
+        by[j] = hit >> j & 1 ? z : by[j];
+    }
 }
 
 // The columns of a warp's hits, in their order, into `list`; how many there are.
@@ -250,11 +265,12 @@ __device__ __forceinline__ void keep_tile(T* kept, const Raw8<T>& raw, int lane)
     }
 }
 
-template <typename T, typename O, int MAP, bool SEEN, int PARTS>
+template <typename T, typename O, int MAP, int MODE, int PARTS>
 __global__ void __launch_bounds__(LOGITS_THREADS, 6)
 process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
-    __shared__ Raw8<T> kept[SEEN ? LOGITS_WARPS : 1][LOGITS_PART * PARTS / 8];
-    __shared__ uint16_t listed[SEEN ? LOGITS_WARPS : 1][LOGITS_PART * PARTS];
+    constexpr bool LIST = MODE == COUNTED;
+    __shared__ Raw8<T> kept[LIST ? LOGITS_WARPS : 1][LOGITS_PART * PARTS / 8];
+    __shared__ uint16_t listed[LIST ? LOGITS_WARPS : 1][LOGITS_PART * PARTS];
     const int lane = threadIdx.x & 31;
     const int base = blockIdx.x * LOGITS_PART * PARTS, left = a.width - base;
 #pragma unroll 1
@@ -267,20 +283,24 @@ process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride)
             load_tile<MAP>(x_row + u * LOGITS_PART, tile_all<MAP>(left - u * LOGITS_PART, lane), lane, x[u]);
         }
         const uint32_t ok = a.allowed ? tile_word<PARTS>(a.allowed + (row * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
-        uint32_t hits = 0;
+        uint32_t seen = 0;
         const int32_t* counts = nullptr;
-        if (SEEN) {
+        if (MODE != NO_HISTORY) {
             const int32_t h = history_of(a, row);
-            hits = tile_hits<PARTS>(a, h, ok, base, left, lane);
-            if (a.counts && h >= 0) counts = a.counts + ((int64_t)h * a.width + base);
+            seen = hit_word<PARTS>(a, h, ok, base, left, lane);
+            if (LIST && h >= 0) counts = a.counts + ((int64_t)h * a.width + base);
         }
-        const bool mend = SEEN && __any_sync(0xffffffffu, hits);
-        T* before = kept[SEEN ? threadIdx.x >> 5 : 0][0].v;
-        uint16_t* list = listed[SEEN ? threadIdx.x >> 5 : 0];
+        T* before = kept[LIST ? threadIdx.x >> 5 : 0][0].v;
+        uint16_t* list = listed[LIST ? threadIdx.x >> 5 : 0];
+        bool mend = false;
         int n_hits = 0, c = 0;                                // c: of this lane's first hit, ahead of time
-        if (mend) {
-            n_hits = list_hits<PARTS>(hits, list, lane);
-            if (counts && lane < n_hits) c = __ldg(counts + list[lane]);
+        if (LIST) {
+            const uint32_t hits = lane_hits<PARTS>(seen, left, lane);
+            mend = __any_sync(0xffffffffu, hits);
+            if (mend) {
+                n_hits = list_hits<PARTS>(hits, list, lane);
+                if (lane < n_hits) c = __ldg(counts + list[lane]);
+            }
         }
         const float* bias = a.bias ? a.bias + (row * a.bias_stride + base) : nullptr;
         O* y_row = out + (row * out_stride + base);
@@ -291,6 +311,10 @@ process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride)
             float y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = as_float(x[u].v[j]);
+            if (MODE == SEEN_ONLY) {
+                const uint32_t hit = tile_bits<MAP>(seen, u, lane);
+                if (hit) penalise_hits(penalty_of(of_row(a.d_repetition, a.repetition, row)), hit, y, y);
+            }
             if (bias) {
                 Raw8<float> b;
                 load_tile<MAP>(bias + u * LOGITS_PART, all, lane, b);
@@ -305,7 +329,7 @@ process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride)
         const float f = of_row(a.d_frequency, a.frequency, row), p = of_row(a.d_presence, a.presence, row);
         for (int i = lane; i < n_hits; i += 32) {
             const int v = list[i], now = c;
-            if (counts && i + 32 < n_hits) c = __ldg(counts + list[i + 32]);
+            if (i + 32 < n_hits) c = __ldg(counts + list[i + 32]);
             const float x1 = as_float(before[v]);
             float y = penalise(pen, x1, x1);
             if (now > 0) y = y - f * (float)now - p;
@@ -317,7 +341,8 @@ process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride)
 }
 
 // The gradients of the logits at a row's hits, over those of its other allowed tokens.  x: the logit of this lane's first hit,
-// fetched ahead of time.
+// fetched ahead of time.  (By the list, because only there are logits read: among all columns, as the repetition penalty of
+// the forward pass, 2,048 x 32,000 took 119 us instead of 83.)
 template <typename T, typename G>
 __device__ __forceinline__ void mend_gradient(const LogitsArgs& a, int row, int n_hits, const uint16_t* list, T x, const T* x_row, const G* g_row, T* d_row, int lane) {
     __syncwarp();                                             // the order of the stores
@@ -348,7 +373,7 @@ logits_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_t gra
             load_tile<MAP>(g_row + u * LOGITS_PART, tile_all<MAP>(left - u * LOGITS_PART, lane), lane, raw[u]);
         }
         const uint32_t ok = a.allowed ? tile_word<PARTS>(a.allowed + (row * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
-        const uint32_t hits = SEEN ? tile_hits<PARTS>(a, history_of(a, row), ok, base, left, lane) : 0;
+        const uint32_t hits = SEEN ? lane_hits<PARTS>(hit_word<PARTS>(a, history_of(a, row), ok, base, left, lane), left, lane) : 0;
         const T* x_row = logits + (row * a.stride + base);
         int n_hits = 0;
         T x = {};
@@ -401,7 +426,7 @@ logits_bias_gradient_kernel(LogitsArgs a, const T* logits, const G* grad, int64_
                 for (int u = 0; u < PARTS; ++u)
                     load_tile<MAP>(grad + (i * grad_stride + base + u * LOGITS_PART), tile_all<MAP>(left - u * LOGITS_PART, lane), lane, raw[k][u]);
                 ok[k] = a.allowed ? tile_word<PARTS>(a.allowed + (i * a.allowed_stride + (base >> 5)), left, lane) : 0xffffffffu;
-                if (SEEN) hits[k] = tile_hits<PARTS>(a, history_of(a, i), ok[k], base, left, lane);
+                if (SEEN) hits[k] = lane_hits<PARTS>(hit_word<PARTS>(a, history_of(a, i), ok[k], base, left, lane), left, lane);
             }
         }
         int n_hits[R] = {};
