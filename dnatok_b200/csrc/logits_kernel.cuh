@@ -86,8 +86,8 @@ process_each_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
 //
 // What bounds it: instructions and memory about alike.  2,048 x 32,000 bf16 to float, a quarter allowed, 5 % seen: 94 us, issue
 // slots 73 % busy, 444 MB = 4.7 TB/s (the counts of scattered tokens cost 64 bytes each from DRAM); 4,096 x 32,000 bf16 with
-// nine tenths allowed: 176 us, 5.3 TB/s; 333 x 32,000 fp16 with the repetition penalty alone 12.4 us, 3.5 TB/s, of
-// which the launch and the first loads are about 4.
+// nine tenths allowed: 176 us, 5.3 TB/s; 333 x 32,000 fp16 with the repetition penalty alone 12.4 us, 3.5 TB/s (one
+// row of 512 takes 4).
 constexpr int LOGITS_PART = 256;
 constexpr int LOGITS_WARPS = LOGITS_THREADS / 32;
 enum { APART, CONTIGUOUS, HALVES };

@@ -63,7 +63,7 @@ def close(got, want, bound, dtype):
     got = host(got)
     with np.errstate(all="ignore"):
         limit = bound + 1.01 * U[dtype] * np.abs(want) + TINY[dtype]
-        same = (got == want) | (np.isnan(got) & np.isnan(want)) | (np.abs(got - want) <= limit)
+        same = (got == want) | (np.isnan(got) & np.isnan(want)) | (np.isfinite(want) & (np.abs(got - want) <= limit))
         # what lies within its error of the largest value of the type may have been rounded to infinity
         top = float(torch.finfo(dtype).max)
         same |= np.isinf(got) & (np.sign(got) == np.sign(want)) & (np.abs(want) + limit >= top)

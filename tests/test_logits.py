@@ -228,6 +228,36 @@ def test_large_calls(n, width, shift, pad, dtype):
     assert torch.equal(dx, g)
 
 
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("n,width,shift,pad", LARGE)
+def test_large_calls_with_the_repetition_penalty_alone(n, width, shift, pad, dtype):
+    """No counts are needed: another kernel than with them.  A hundredth of the logits are no ordinary numbers."""
+    d = make(n, width, dtype, seed=29, shift=shift, pad=pad, history_rows=n if n < 1000 else 50)
+    rng = np.random.default_rng(31)
+    odd = torch.from_numpy(rng.choice(np.array([np.nan, np.inf, -np.inf, 0.0, -0.0]), (n, width)))
+    d["x"].copy_(torch.where(torch.from_numpy(rng.random((n, width)) < 0.01).cuda(), odd.to(dtype).cuda(), d["x"]))
+    target = rng.integers(-5, 55, n) if n >= 1000 else rng.permutation(n)
+    inside = (target >= 0) & (target < len(d["seen"]))
+    seen, rows = d["seen"][np.where(inside, target, 0)] & inside[:, None], torch.from_numpy(target).cuda()
+    x = R.host(d["x"])
+    pen, ref = dict(history=d["h"], rows=rows, repetition=cuda(d["r"])), dict(seen=seen, r=d["r"])
+    for out_dtype in {dtype, torch.float32}:
+        for kw, more in [(pen, ref),
+                         (dict(allowed=words(d["ok"]), **pen), dict(ok=d["ok"], **ref)),
+                         (dict(bias=cuda(d["bias"]), allowed=words(d["ok"][:1])[0], **pen), dict(bias=d["bias"], ok=np.broadcast_to(d["ok"][:1], (n, width)), **ref)),
+                         (dict(bias=cuda(d["bias"][0]), **pen), dict(bias=d["bias"][:1], **ref))]:
+            want, bound = R.logits(x, **more)
+            y = process_logits(d["x"], out_dtype=out_dtype, **kw)
+            R.close(y, want, bound, out_dtype)
+            if kw is pen:
+                zeros = want == 0
+                assert (np.signbit(R.host(y))[zeros] == np.signbit(want)[zeros]).all()
+            if out_dtype == dtype and shift == 0:
+                z = d["x"].clone()
+                process_logits(z, out=z, **kw)
+                R.close(z, R.host(y), 0.0, dtype)
+
+
 def test_offsets_beyond_32_bits():
     """70,001 x 32,000 logits and a history as large: the last rows as in a call of their own."""
     n, width, last = 70001, 32000, 3
