@@ -19,9 +19,10 @@ after its chosen token.  A generation loop:
 Everything numeric happens in ``libdnatok_b200.so``; work is enqueued on the current stream of the tensors' device and
 nothing waits for it.  Sets of tokens are int32 words: bit ``v % 32`` of word ``v // 32`` stands for token ``v``.
 
-The calls can be captured into a CUDA graph (use a ``Grammar`` on the device once before).  To capture a gradient while an
-eager graph over the same leaf tensors is alive, call ``process_logits_backward``, which needs no autograd graph:
-autograd's own accumulation into a leaf waits on the stream of the older graph, which a capture does not allow.
+The calls can be captured into a CUDA graph (use a ``Grammar`` on the device once before, and keep it as long as the graph).
+To capture a gradient while an eager graph over the same leaf tensors is alive, call ``process_logits_backward``, which needs
+no autograd graph: autograd's own accumulation into a leaf waits on the stream of the older graph, which a capture does not
+allow.
 """
 from __future__ import annotations
 

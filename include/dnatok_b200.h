@@ -358,6 +358,7 @@ typedef struct dnatok_grammar dnatok_grammar;
 int dnatok_create_grammar(const int32_t* next, int32_t n_states, int32_t n_classes, const uint8_t* accepting,
                           const uint8_t byte_class[256], const uint8_t* token_bytes, const int64_t* token_offsets,
                           int64_t width, int64_t end_id, dnatok_grammar** out);
+/* Frees its tables on the devices too: not before the last replay of a CUDA graph that holds calls with it. */
 void dnatok_destroy_grammar(dnatok_grammar* g);
 
 /* d_allowed[row] = the tokens whose bytes lead from d_states[row] to a live state; the end token where the state accepts
