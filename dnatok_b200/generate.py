@@ -326,8 +326,6 @@ def _penalty(name: str, v, n: int, dev: int):
         _on(v, name, dev)
         if v.dtype is not torch.float32 or v.shape != (n,) or (n > 1 and v.stride(0) != 1):
             raise ValueError("%s must be a number or a contiguous float32 tensor [%d]" % (name, n))
-        if v.requires_grad and torch.is_grad_enabled():
-            raise ValueError("%s has no gradient" % name)
         return neutral, v.data_ptr(), True
     v = float(v)
     if neutral:
@@ -483,9 +481,14 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
     * ``allowed`` int32 [n, words] or [words]: tokens whose bit is 0 become ``-inf`` whatever their logits hold, NaN
       included.  A row without an allowed token is ``-inf`` throughout.
 
-    All of it is computed in 32 bits and rounded once.  Differentiable in ``logits`` and ``bias``; the history and the mask
-    must then stay as they are until the backward pass (autograd refuses it otherwise)."""
-    if (getattr(logits, "requires_grad", False) or (bias is not None and getattr(bias, "requires_grad", False))) and torch.is_grad_enabled():
+    All of it is computed in 32 bits and rounded once.  Differentiable in ``logits`` and ``bias`` (a penalty that requires a
+    gradient is refused); the history and the mask must then stay as they are until the backward pass (autograd refuses it otherwise)."""
+    recording = torch.is_grad_enabled()
+    if recording:                                    # (here: inside of an autograd function the mode is off)
+        for name, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+            if isinstance(v, torch.Tensor) and v.requires_grad:
+                raise ValueError("%s has no gradient" % name)
+    if recording and (getattr(logits, "requires_grad", False) or (bias is not None and getattr(bias, "requires_grad", False))):
         if out is not None:
             raise ValueError("out= has no gradient; leave it out or call under torch.no_grad()")
         return _Process.apply(logits, bias, history, rows, repetition, frequency, presence, allowed, out_dtype)

@@ -1,0 +1,22 @@
+"""What autograd and tracing may make of the operators around logits (refused where they would be wrong without a word)."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from dnatok_b200 import process_logits  # noqa: E402
+
+from generate_host import history, library  # noqa: E402,F401
+
+
+@pytest.mark.parametrize("name", ["repetition", "frequency", "presence"])
+@pytest.mark.parametrize("leaf", ["logits", "bias", "neither"])
+def test_a_penalty_that_needs_a_gradient_is_refused(library, name, leaf):  # noqa: F811
+    x, b = torch.randn(3, 40, requires_grad=leaf == "logits"), torch.randn(40, requires_grad=leaf == "bias")
+    h, v = history(3, 40), torch.ones(3, requires_grad=True)
+    with pytest.raises(ValueError, match="%s has no gradient" % name):
+        process_logits(x, history=h, bias=b, **{name: v})
+    assert not library.calls
+    with torch.no_grad():
+        process_logits(x, history=h, bias=b, **{name: v})
+    process_logits(x, history=h, bias=b, **{name: v.detach()})
+    assert [c[0] for c in library.calls] == ["dnatok_process_logits"] * 2
