@@ -488,6 +488,8 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
         for name, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
             if isinstance(v, torch.Tensor) and v.requires_grad:
                 raise ValueError("%s has no gradient" % name)
+        if getattr(out, "requires_grad", False):
+            raise ValueError("out= has no gradient; leave it out or call under torch.no_grad()")
     if recording and (getattr(logits, "requires_grad", False) or (bias is not None and getattr(bias, "requires_grad", False))):
         if out is not None:
             raise ValueError("out= has no gradient; leave it out or call under torch.no_grad()")

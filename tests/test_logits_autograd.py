@@ -20,3 +20,15 @@ def test_a_penalty_that_needs_a_gradient_is_refused(library, name, leaf):  # noq
         process_logits(x, history=h, bias=b, **{name: v})
     process_logits(x, history=h, bias=b, **{name: v.detach()})
     assert [c[0] for c in library.calls] == ["dnatok_process_logits"] * 2
+
+
+@pytest.mark.parametrize("leaf", [True, False])
+def test_an_output_that_is_part_of_a_graph_is_refused(library, leaf):  # noqa: F811
+    """Its new values would not be those that its graph differentiates."""
+    x, w = torch.randn(3, 40), torch.randn(3, 40, requires_grad=True)
+    out = w if leaf else w * 2
+    with pytest.raises(ValueError, match="out= has no gradient"):
+        process_logits(x, out=out)
+    assert not library.calls and (leaf or out.grad_fn is not None)
+    with torch.no_grad():
+        assert process_logits(x, out=out) is out
