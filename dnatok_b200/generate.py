@@ -31,6 +31,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 from .automaton import Automaton
@@ -41,6 +42,11 @@ _BITS = {torch.int32: 32, torch.int64: 64}
 
 Number = Union[float, int, torch.Tensor]
 _LEAST, _MOST = 2.0 ** -126, 2.0 ** 126              # a repetition penalty whose reciprocal is a normal number too
+
+
+# The open level of forward-mode differentiation, -1 for none (the public ``unpack_dual`` asks for each tensor: 0.5 us apiece).
+def _forward_level() -> int:
+    return getattr(forward_ad, "_current_level", 0)
 
 
 # The current stream of a device as a number (the public call builds a Stream object on the way: 2 us instead of 0.1).
@@ -76,6 +82,13 @@ def _call(fn, dev: int, *args) -> None:
             rc = fn(*args, _raw_stream(dev))
     if rc:
         _cabi.check(rc)
+
+
+def _no_tangents(**named) -> None:
+    """Forward mode would read a result without a tangent as one that does not change."""
+    for name, t in named.items():
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("%s has a tangent; there is no forward-mode derivative" % name)
 
 
 def _written(t: torch.Tensor) -> None:
@@ -482,7 +495,10 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
       included.  A row without an allowed token is ``-inf`` throughout.
 
     All of it is computed in 32 bits and rounded once.  Differentiable in ``logits`` and ``bias`` (a penalty that requires a
-    gradient is refused); the history and the mask must then stay as they are until the backward pass (autograd refuses it otherwise)."""
+    gradient is refused, and so is forward mode); the history and the mask must then stay as they are until the backward pass
+    (autograd refuses it otherwise)."""
+    if _forward_level() >= 0:
+        _no_tangents(logits=logits, repetition=repetition, frequency=frequency, presence=presence, bias=bias, out=out)
     recording = torch.is_grad_enabled()
     if recording:                                    # (here: inside of an autograd function the mode is off)
         for name, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
@@ -505,6 +521,8 @@ def process_logits_backward(grad, logits, *, history: Optional[TokenHistory] = N
                             frequency: Number = 0.0, presence: Number = 0.0, bias=None, allowed=None):
     """(gradient of ``logits``, gradient of ``bias`` or None) for ``grad``, the gradient of ``process_logits`` called with the
     same arguments; without autograd."""
+    if _forward_level() >= 0:
+        _no_tangents(grad=grad, logits=logits, repetition=repetition, frequency=frequency, presence=presence, bias=bias)
     with torch.no_grad():
         a, dev = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
         _on(grad, "grad", dev)

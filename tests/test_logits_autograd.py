@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from dnatok_b200 import process_logits  # noqa: E402
+from dnatok_b200 import process_logits, process_logits_backward  # noqa: E402
 
 from generate_host import history, library  # noqa: E402,F401
 
@@ -32,3 +32,28 @@ def test_an_output_that_is_part_of_a_graph_is_refused(library, leaf):  # noqa: F
     assert not library.calls and (leaf or out.grad_fn is not None)
     with torch.no_grad():
         assert process_logits(x, out=out) is out
+
+
+@pytest.mark.parametrize("name", ["logits", "bias", "repetition", "frequency", "presence"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(library, name, grad):  # noqa: F811
+    from torch.autograd import forward_ad
+    args = {"logits": torch.randn(3, 40, requires_grad=grad), "bias": torch.randn(40), "repetition": torch.ones(3), "frequency": torch.ones(3),
+            "presence": torch.ones(3)}
+    h = history(3, 40)
+    with forward_ad.dual_level():
+        dual = dict(args)
+        dual[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(RuntimeError, match="%s has a tangent" % name):
+            process_logits(history=h, **dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="%s has a tangent" % name):
+            process_logits(history=h, **dual)
+        with pytest.raises(RuntimeError, match="%s has a tangent" % name):
+            process_logits_backward(torch.ones(3, 40), history=h, **dual)
+        assert not library.calls
+        process_logits(history=h, **args)                          # no tangent anywhere: nothing is lost
+        with pytest.raises(RuntimeError, match="grad has a tangent"):
+            process_logits_backward(forward_ad.make_dual(torch.ones(3, 40), torch.ones(3, 40)), args["logits"])
+        with torch.no_grad(), pytest.raises(RuntimeError, match="out has a tangent"):
+            process_logits(args["logits"], out=forward_ad.make_dual(torch.ones(3, 40), torch.ones(3, 40)))
+    assert [c[0] for c in library.calls] == ["dnatok_process_logits"]
