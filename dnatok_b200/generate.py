@@ -17,7 +17,7 @@ after its chosen token.  A generation loop:
         states, allowed = grammar.step(states, tokens)
 
 Everything numeric happens in ``libdnatok_b200.so``; work is enqueued on the current stream of the tensors' device and
-nothing waits for it.  Sets of tokens are int32 words: bit ``v % 32`` of word ``v // 32`` stands for token ``v``.
+nothing waits for it.  (``torch.jit.trace`` and ``make_fx`` cannot record that work: the calls refuse to be traced.)  Sets of tokens are int32 words: bit ``v % 32`` of word ``v // 32`` stands for token ``v``.
 
 The calls can be captured into a CUDA graph (use a ``Grammar`` on the device once before, and keep it as long as the graph).
 To capture a gradient while an eager graph over the same leaf tensors is alive, call ``process_logits_backward``, which needs
@@ -27,6 +27,7 @@ allow.
 from __future__ import annotations
 
 import ctypes
+import sys
 from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -73,8 +74,16 @@ def _on(t, what: str, dev: int) -> None:
         raise ValueError("%s is on cuda:%d, the call on cuda:%d" % (what, d, dev))
 
 
+def _traced() -> bool:
+    """Whether ``torch.jit.trace`` or ``make_fx`` is recording the operations of this thread."""
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    return torch.jit.is_tracing() or (proxies is not None and proxies.get_proxy_mode() is not None)
+
+
 def _call(fn, dev: int, *args) -> None:
     """A C entry point with the device current and its current stream as the last argument."""
+    if _traced():                                    # (the trace would hold the output's allocation and nothing that fills it)
+        raise RuntimeError("kernels of this library cannot be recorded by torch.jit.trace or make_fx")
     if torch.cuda.current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:

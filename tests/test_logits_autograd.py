@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from dnatok_b200 import process_logits, process_logits_backward  # noqa: E402
+from dnatok_b200 import Automaton, Grammar, process_logits, process_logits_backward  # noqa: E402
 
 from generate_host import history, library  # noqa: E402,F401
 
@@ -57,3 +57,28 @@ def test_forward_mode_is_refused(library, name, grad):  # noqa: F811
         with torch.no_grad(), pytest.raises(RuntimeError, match="out has a tangent"):
             process_logits(args["logits"], out=forward_ad.make_dual(torch.ones(3, 40), torch.ones(3, 40)))
     assert [c[0] for c in library.calls] == ["dnatok_process_logits"]
+
+
+CALLS = {"process_logits": lambda x, h, g: process_logits(x, history=h, repetition=1.5),
+         "process_logits_backward": lambda x, h, g: process_logits_backward(x, x, history=h, repetition=1.5)[0],
+         "add": lambda x, h, g: (h.add(x.long()), x)[1],
+         "append": lambda x, h, g: (h.append(x[:, 0].long()), x)[1],
+         "allowed": lambda x, h, g: g.allowed(x[:, 0].int()),
+         "advance": lambda x, h, g: g.advance(x[:, 0].int(), x[:, 1].long()),
+         "step": lambda x, h, g: g.step(x[:, 0].int(), x[:, 1].long())[1]}
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("call", CALLS)
+def test_traces_are_refused(library, call):  # noqa: F811
+    """They would hold the allocation of the output and nothing that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    h, g = history(3, 40), Grammar(Automaton.avoiding(["ACG"]), [b"A", b"C"] * 20)
+    library.calls.clear()
+    x = torch.zeros(3, 40)
+    for trace in (lambda f: torch.jit.trace(f, x, check_trace=False), lambda f: make_fx(f)(x), lambda f: make_fx(f, pre_dispatch=True)(x)):
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            trace(lambda z: CALLS[call](z, h, g))
+        assert not library.calls
+    CALLS[call](x, h, g)                                           # and nothing is left of it
+    assert len(library.calls) == 1
