@@ -17,7 +17,8 @@ after its chosen token.  A generation loop:
         states, allowed = grammar.step(states, tokens)
 
 Everything numeric happens in ``libdnatok_b200.so``; work is enqueued on the current stream of the tensors' device and
-nothing waits for it.  (``torch.jit.trace`` and ``make_fx`` cannot record that work: the calls refuse to be traced.)  Sets of tokens are int32 words: bit ``v % 32`` of word ``v // 32`` stands for token ``v``.
+nothing waits for it.  (``torch.jit.trace`` and ``make_fx`` cannot record that work: the calls refuse to be traced.)
+Sets of tokens are int32 words: bit ``v % 32`` of word ``v // 32`` stands for token ``v``.
 
 The calls can be captured into a CUDA graph (use a ``Grammar`` on the device once before, and keep it as long as the graph).
 To capture a gradient while an eager graph over the same leaf tensors is alive, call ``process_logits_backward``, which needs
@@ -358,9 +359,9 @@ def _penalty(name: str, v, n: int, dev: int):
     return v, None, v != neutral
 
 
-def _shared(t) -> bool:
+def _shared(shape) -> bool:
     """Whether an array of one row, or without rows, stands for all of them."""
-    return t.dim() == 1 or t.shape[0] == 1
+    return len(shape) == 1 or shape[0] == 1
 
 
 def _row_array(t, what: str, dtype, n: int, columns: int, dev: int) -> Tuple[int, int]:
@@ -439,15 +440,16 @@ def _forward(a, dev: int, out):
     return out
 
 
-def _backward(a, dev: int, logits, grad, bias, want_logits: bool, want_bias: bool):
+def _backward(a, dev: int, logits, grad, bias_shape, want_logits: bool):
+    """(gradient of the logits, if wanted, gradient of a bias of ``bias_shape``, if that is not None)."""
     if grad.shape[1] > 1 and grad.stride(1) != 1:
         grad = grad.contiguous()
     n, width = grad.shape
     L = _cabi.lib()
     dx = logits.new_empty((n, width)) if want_logits else None
     db, scratch, need = None, None, 0
-    if want_bias:
-        db = bias.new_empty(bias.shape)
+    if bias_shape is not None:
+        db = grad.new_empty(bias_shape, dtype=torch.float32)
         if a.bias_stride == 0:
             need = L.dnatok_logits_scratch_bytes(n, width)
             if need:
@@ -463,7 +465,8 @@ class _Process(torch.autograd.Function):
     def forward(ctx, logits, bias, history, rows, repetition, frequency, presence, allowed, out_dtype):
         a, dev = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
         out = _forward(a, dev, _output(logits, None, out_dtype))
-        ctx.save_for_backward(logits, bias, rows if a.rows else None, allowed, history.seen if a.seen else None,
+        ctx.bias_shape = None if bias is None else bias.shape     # (its values have no part in the gradients)
+        ctx.save_for_backward(logits, rows if a.rows else None, allowed, history.seen if a.seen else None,
                               repetition if isinstance(repetition, torch.Tensor) else None)
         ctx.number = a.repetition
         return out
@@ -472,7 +475,7 @@ class _Process(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         # (the tensors may have been stored elsewhere in the meantime: nothing but them holds for their addresses)
-        logits, bias, rows, allowed, seen, repetition = ctx.saved_tensors
+        logits, rows, allowed, seen, repetition = ctx.saved_tensors
         a = _cabi.Logits()
         a.logits, a.dtype, a.stride = logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0)
         a.n_rows, a.width = logits.shape
@@ -484,10 +487,11 @@ class _Process(torch.autograd.Function):
         if rows is not None:
             a.rows, a.rows_bits = rows.data_ptr(), _BITS[rows.dtype]
         if allowed is not None:
-            a.allowed, a.allowed_stride = allowed.data_ptr(), 0 if _shared(allowed) else allowed.stride(0)
-        if bias is not None and not _shared(bias):
+            a.allowed, a.allowed_stride = allowed.data_ptr(), 0 if _shared(allowed.shape) else allowed.stride(0)
+        bias_shape = ctx.bias_shape if ctx.needs_input_grad[1] else None
+        if bias_shape is not None and not _shared(bias_shape):
             a.bias_stride = a.width
-        dx, db = _backward(a, logits.get_device(), logits, grad, bias, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        dx, db = _backward(a, logits.get_device(), logits, grad, bias_shape, ctx.needs_input_grad[0])
         return dx, db, None, None, None, None, None, None, None
 
 
@@ -537,6 +541,6 @@ def process_logits_backward(grad, logits, *, history: Optional[TokenHistory] = N
         _on(grad, "grad", dev)
         if grad.dim() != 2 or grad.shape != logits.shape or grad.dtype not in (logits.dtype, torch.float32):
             raise ValueError("grad must be a tensor %r of the logits' type or float32" % (tuple(logits.shape),))
-        if bias is not None and not _shared(bias):
+        if bias is not None and not _shared(bias.shape):
             a.bias_stride = a.width
-        return _backward(a, dev, logits, grad, bias, True, bias is not None)
+        return _backward(a, dev, logits, grad, None if bias is None else bias.shape, True)

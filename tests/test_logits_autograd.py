@@ -82,3 +82,14 @@ def test_traces_are_refused(library, call):  # noqa: F811
         assert not library.calls
     CALLS[call](x, h, g)                                           # and nothing is left of it
     assert len(library.calls) == 1
+
+
+def test_a_bias_may_change_before_the_backward_pass(library):  # noqa: F811
+    """Its gradient does not depend on its values: an optimiser may step in between."""
+    for shape in ((40,), (1, 40), (3, 40)):
+        x, b = torch.randn(3, 40, requires_grad=True), torch.randn(shape, requires_grad=True)
+        y = process_logits(x, bias=b)
+        with torch.no_grad():
+            b.add_(1)
+        dx, db = torch.autograd.grad(y, (x, b), torch.ones(3, 40))
+        assert db.shape == b.shape and db.dtype == torch.float32 and db.is_contiguous()
