@@ -440,20 +440,21 @@ def _forward(a, dev: int, out):
     return out
 
 
-def _backward(a, dev: int, logits, grad, bias_shape, want_logits: bool):
-    """(gradient of the logits, if wanted, gradient of a bias of ``bias_shape``, if that is not None)."""
+def _backward(a, dev: int, dtype, grad, bias_shape, want_logits: bool):
+    """(gradient of logits of ``dtype``, if wanted, gradient of a bias of ``bias_shape``, if that is not None)."""
     if grad.shape[1] > 1 and grad.stride(1) != 1:
         grad = grad.contiguous()
     n, width = grad.shape
     L = _cabi.lib()
-    dx = logits.new_empty((n, width)) if want_logits else None
+    dx = grad.new_empty((n, width), dtype=dtype) if want_logits else None
     db, scratch, need = None, None, 0
     if bias_shape is not None:
         db = grad.new_empty(bias_shape, dtype=torch.float32)
-        if a.bias_stride == 0:
+        a.bias_stride = 0 if _shared(bias_shape) else width
+        if _shared(bias_shape):
             need = L.dnatok_logits_scratch_bytes(n, width)
             if need:
-                scratch = logits.new_empty((need,), dtype=torch.uint8)
+                scratch = grad.new_empty((need,), dtype=torch.uint8)
     _call(L.dnatok_process_logits_backward, dev, a, grad.data_ptr(), _TYPES[grad.dtype], grad.stride(0),
           dx.data_ptr() if dx is not None else None, width, db.data_ptr() if db is not None else None,
           scratch.data_ptr() if need else None, need)
@@ -465,33 +466,36 @@ class _Process(torch.autograd.Function):
     def forward(ctx, logits, bias, history, rows, repetition, frequency, presence, allowed, out_dtype):
         a, dev = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)
         out = _forward(a, dev, _output(logits, None, out_dtype))
+        ctx.dtype = logits.dtype
         ctx.bias_shape = None if bias is None else bias.shape     # (its values have no part in the gradients)
-        ctx.save_for_backward(logits, rows if a.rows else None, allowed, history.seen if a.seen else None,
-                              repetition if isinstance(repetition, torch.Tensor) else None)
-        ctx.number = a.repetition
+        ctx.number = 1.0 if isinstance(repetition, torch.Tensor) else float(repetition)
+        # The logits' signs, and the history, matter to the gradient of penalised logits alone.
+        if history is not None and ctx.needs_input_grad[0] and (isinstance(repetition, torch.Tensor) or ctx.number != 1.0):
+            ctx.save_for_backward(allowed, logits, history.seen, rows, repetition if isinstance(repetition, torch.Tensor) else None)
+        else:
+            ctx.save_for_backward(allowed, None, None, None, None)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         # (the tensors may have been stored elsewhere in the meantime: nothing but them holds for their addresses)
-        logits, rows, allowed, seen, repetition = ctx.saved_tensors
+        allowed, logits, seen, rows, repetition = ctx.saved_tensors
         a = _cabi.Logits()
-        a.logits, a.dtype, a.stride = logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0)
-        a.n_rows, a.width = logits.shape
-        a.repetition = ctx.number
-        if repetition is not None:
-            a.d_repetition = repetition.data_ptr()
-        if seen is not None:
+        a.dtype, a.repetition = _TYPES[ctx.dtype], ctx.number
+        a.n_rows, a.width = grad.shape
+        if logits is None:
+            a.logits = grad.data_ptr()               # not read: no token counts as seen
+        else:
+            a.logits, a.stride = logits.data_ptr(), logits.stride(0)
             a.seen, a.history_rows = seen.data_ptr(), seen.shape[0]
-        if rows is not None:
-            a.rows, a.rows_bits = rows.data_ptr(), _BITS[rows.dtype]
+            if rows is not None:
+                a.rows, a.rows_bits = rows.data_ptr(), _BITS[rows.dtype]
+            if repetition is not None:
+                a.d_repetition = repetition.data_ptr()
         if allowed is not None:
             a.allowed, a.allowed_stride = allowed.data_ptr(), 0 if _shared(allowed.shape) else allowed.stride(0)
-        bias_shape = ctx.bias_shape if ctx.needs_input_grad[1] else None
-        if bias_shape is not None and not _shared(bias_shape):
-            a.bias_stride = a.width
-        dx, db = _backward(a, logits.get_device(), logits, grad, bias_shape, ctx.needs_input_grad[0])
+        dx, db = _backward(a, grad.get_device(), ctx.dtype, grad, ctx.bias_shape if ctx.needs_input_grad[1] else None, ctx.needs_input_grad[0])
         return dx, db, None, None, None, None, None, None, None
 
 
@@ -541,6 +545,4 @@ def process_logits_backward(grad, logits, *, history: Optional[TokenHistory] = N
         _on(grad, "grad", dev)
         if grad.dim() != 2 or grad.shape != logits.shape or grad.dtype not in (logits.dtype, torch.float32):
             raise ValueError("grad must be a tensor %r of the logits' type or float32" % (tuple(logits.shape),))
-        if bias is not None and not _shared(bias.shape):
-            a.bias_stride = a.width
-        return _backward(a, dev, logits, grad, None if bias is None else bias.shape, True)
+        return _backward(a, dev, logits.dtype, grad, None if bias is None else bias.shape, True)

@@ -93,3 +93,47 @@ def test_a_bias_may_change_before_the_backward_pass(library):  # noqa: F811
             b.add_(1)
         dx, db = torch.autograd.grad(y, (x, b), torch.ones(3, 40))
         assert db.shape == b.shape and db.dtype == torch.float32 and db.is_contiguous()
+
+
+def test_without_a_repetition_penalty_nothing_but_the_mask_is_kept(library):  # noqa: F811
+    """Frequency, presence and bias have derivatives that depend on no logit and no history: both may change."""
+    for kw in (dict(frequency=0.5), dict(presence=torch.ones(3), repetition=1.0), {}):
+        w, b = torch.randn(3, 40, requires_grad=True), torch.randn(40, requires_grad=True)
+        x, h, ok, rows = w * 2, history(3, 40), torch.zeros((3, 2), dtype=torch.int32), torch.arange(3)
+        y = process_logits(x, history=h, rows=rows, bias=b, allowed=ok, **kw)
+        h.append(torch.zeros(3, dtype=torch.int64))
+        rows.zero_()
+        with torch.no_grad():
+            x.mul_(2)
+        library.calls.clear()
+        dw, db = torch.autograd.grad(y, (w, b), torch.ones(3, 40))
+        a = library.calls[-1][1]
+        assert library.calls[-1][0] == "dnatok_process_logits_backward"
+        assert (a.n_rows, a.width, a.dtype, a.seen, a.rows, a.allowed) == (3, 40, 0, None, None, ok.data_ptr()) and a.logits
+        assert dw.shape == (3, 40) and db.shape == (40,)
+        y = process_logits(x, history=h, allowed=ok, **kw)
+        ok.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+@pytest.mark.parametrize("change", ["logits", "seen", "rows", "repetition"])
+def test_what_the_repetition_penalty_depends_on_stays(library, change):  # noqa: F811
+    w, h, rows, r = torch.randn(3, 40, requires_grad=True), history(3, 40), torch.arange(3), torch.ones(3)
+    x = w * 2
+    y = process_logits(x, history=h, rows=rows, repetition=r)
+    with torch.no_grad():
+        {"logits": x, "seen": h.seen, "rows": rows, "repetition": r}[change].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_a_bias_alone_keeps_no_logits(library):  # noqa: F811
+    x, h, r = torch.randn(3, 40), history(3, 40), torch.ones(3)
+    b = torch.randn(40, requires_grad=True)
+    y = process_logits(x, history=h, repetition=r, bias=b)
+    x.zero_()
+    r.zero_()
+    h.append(torch.zeros(3, dtype=torch.int64))
+    db, = torch.autograd.grad(y, b, torch.ones(3, 40))
+    assert db.shape == (40,) and library.calls[-1][1].seen is None
