@@ -75,6 +75,14 @@ def _on(t, what: str, dev: int) -> None:
         raise ValueError("%s is on cuda:%d, the call on cuda:%d" % (what, d, dev))
 
 
+def _address(t: torch.Tensor, what: str) -> int:
+    """Where a tensor's elements are; 0 is no argument to the library, so only a tensor without elements may give it."""
+    p = t.data_ptr()
+    if not p and t.numel():
+        raise ValueError("%s has no memory of its own (a distributed, fake or otherwise wrapped tensor)" % what)
+    return p
+
+
 def _traced() -> bool:
     """Whether ``torch.jit.trace`` or ``make_fx`` is recording the operations of this thread."""
     proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
@@ -181,7 +189,7 @@ class TokenHistory:
             if offsets.dtype is not torch.int64 or offsets.dim() != 1 or offsets.shape[0] < 1 or not offsets.is_contiguous():
                 raise ValueError("offsets must be a contiguous int64 tensor [n + 1]")
             n = offsets.shape[0] - 1
-            h.offsets, h.total = offsets.data_ptr(), ids.shape[0]
+            h.offsets, h.total = _address(offsets, "offsets"), ids.shape[0]
         else:
             if ids.dim() != 2 or (ids.shape[1] > 1 and ids.stride(1) != 1):
                 raise ValueError("padded ids must be a tensor [n, T] whose rows are contiguous")
@@ -191,7 +199,7 @@ class TokenHistory:
                 _on(lengths, "lengths", dev)
                 if lengths.dtype is not torch.int32 or lengths.shape != (n,) or not lengths.is_contiguous():
                     raise ValueError("lengths must be a contiguous int32 tensor [%d]" % n)
-                h.lengths = lengths.data_ptr()
+                h.lengths = _address(lengths, "lengths")
             h.pad_left = 1 if pad_left else 0
         self._enter(h, ids, n, rows, generated, dev)
 
@@ -208,13 +216,13 @@ class TokenHistory:
     def _enter(self, h, ids, n: int, rows, generated: bool, dev: int) -> None:
         if rows is not None:
             h.rows_bits = _tokens(rows, "rows", n, dev)
-            h.rows = rows.data_ptr()
+            h.rows = _address(rows, "rows")
         elif n != self.n_rows:
             raise ValueError("the history has %d rows, the call %d" % (self.n_rows, n))
-        h.seen, h.history_rows, h.width = self.seen.data_ptr(), self.n_rows, self.width
+        h.seen, h.history_rows, h.width = _address(self.seen, "seen"), self.n_rows, self.width
         if self.counts is not None:
-            h.counts = self.counts.data_ptr()
-        h.ids, h.id_bits, h.n_rows = ids.data_ptr(), _BITS[ids.dtype], n
+            h.counts = _address(self.counts, "counts")
+        h.ids, h.id_bits, h.n_rows = _address(ids, "ids"), _BITS[ids.dtype], n
         _call(_cabi.lib().dnatok_history_add, dev, h, 1 if generated else 0)
         _written(self.seen)
         if generated and self.counts is not None:
@@ -274,11 +282,12 @@ class Grammar:
                           device=torch.device("cuda" if device is None else device))
 
     @staticmethod
-    def _states(states) -> Tuple[int, int]:
+    def _states(states) -> Tuple[int, int, int]:
+        """(how many, the number of their GPU, their address)."""
         dev = _device_of(states, "states")
         if states.dtype is not torch.int32 or states.dim() != 1 or (states.shape[0] > 1 and states.stride(0) != 1):
             raise ValueError("states must be a contiguous int32 tensor [n]")
-        return states.shape[0], dev
+        return states.shape[0], dev, _address(states, "states")
 
     def _mask(self, states, n: int, dev: int, out):
         words = _words(self.width)
@@ -300,9 +309,9 @@ class Grammar:
 
     def allowed(self, states, *, out=None) -> torch.Tensor:
         """int32 [n, words]: the tokens that may follow in each state."""
-        n, dev = self._states(states)
+        n, dev, at = self._states(states)
         mask = self._mask(states, n, dev, out)
-        _call(_cabi.lib().dnatok_grammar_allowed, dev, self.ptr, states.data_ptr(), n, mask.data_ptr())
+        _call(_cabi.lib().dnatok_grammar_allowed, dev, self.ptr, at, n, _address(mask, "the mask"))
         if out is not None:
             _written(out)
         return mask
@@ -310,21 +319,23 @@ class Grammar:
     def advance(self, states, tokens, *, out=None) -> torch.Tensor:
         """int32 [n]: the states after ``tokens`` [n] (int32 or int64); a token outside the vocabulary (-1, say) leaves its
         row as it was.  ``out`` may be ``states``."""
-        n, dev = self._states(states)
+        n, dev, at = self._states(states)
         bits = _tokens(tokens, "tokens", n, dev)
         new = self._new_states(states, n, dev, out)
-        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, states.data_ptr(), tokens.data_ptr(), bits, n, new.data_ptr(), None)
+        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, at, _address(tokens, "tokens"), bits, n,
+              _address(new, "out"), None)
         if out is not None:
             _written(out)
         return new
 
     def step(self, states, tokens, *, out=None, out_allowed=None) -> Tuple[torch.Tensor, torch.Tensor]:
         """``advance`` and the masks of the new states in one call: (states, allowed).  ``out`` may not be ``states``."""
-        n, dev = self._states(states)
+        n, dev, at = self._states(states)
         bits = _tokens(tokens, "tokens", n, dev)
         new = self._new_states(states, n, dev, out)
         mask = self._mask(states, n, dev, out_allowed)
-        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, states.data_ptr(), tokens.data_ptr(), bits, n, new.data_ptr(), mask.data_ptr())
+        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, at, _address(tokens, "tokens"), bits, n,
+              _address(new, "out"), _address(mask, "the mask"))
         if out is not None:
             _written(out)
         if out_allowed is not None:
@@ -349,7 +360,7 @@ def _penalty(name: str, v, n: int, dev: int):
         _on(v, name, dev)
         if v.dtype is not torch.float32 or v.shape != (n,) or (n > 1 and v.stride(0) != 1):
             raise ValueError("%s must be a number or a contiguous float32 tensor [%d]" % (name, n))
-        return neutral, v.data_ptr(), True
+        return neutral, _address(v, name), True
     v = float(v)
     if neutral:
         if not _LEAST <= v <= _MOST:
@@ -373,10 +384,10 @@ def _row_array(t, what: str, dtype, n: int, columns: int, dev: int) -> Tuple[int
             or (len(shape) == 2 and shape[0] != 1 and shape[0] != n):
         raise ValueError("%s must be a %s tensor [%d, %d] or [%d] whose rows are contiguous" % (what, str(dtype)[6:], n, columns, columns))
     if len(shape) == 1 or shape[0] == 1:
-        return t.data_ptr(), 0
+        return _address(t, what), 0
     if strides[0] < columns:
         raise ValueError("rows of %s overlap" % what)
-    return t.data_ptr(), strides[0]
+    return _address(t, what), strides[0]
 
 
 def _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed):
@@ -387,7 +398,7 @@ def _arguments(logits, history, rows, repetition, frequency, presence, bias, all
     if dtype is None:
         raise ValueError("logits must be float32, float16 or bfloat16")
     a = _cabi.Logits()
-    a.logits, a.dtype, a.n_rows, a.width, a.stride = logits.data_ptr(), dtype, n, width, stride
+    a.logits, a.dtype, a.n_rows, a.width, a.stride = _address(logits, "logits"), dtype, n, width, stride
     a.repetition, a.d_repetition, once = _penalty("repetition", repetition, n, dev)
     a.frequency, a.d_frequency, often = _penalty("frequency", frequency, n, dev)
     a.presence, a.d_presence, also = _penalty("presence", presence, n, dev)
@@ -404,15 +415,15 @@ def _arguments(logits, history, rows, repetition, frequency, presence, bias, all
             raise ValueError("the history is on %s, the logits on %s" % (history.device, logits.device))
         if rows is not None:
             a.rows_bits = _tokens(rows, "rows", n, dev)
-            a.rows = rows.data_ptr()
+            a.rows = _address(rows, "rows")
         elif history.n_rows != n:
             raise ValueError("the history has %d rows, the logits %d" % (history.n_rows, n))
         if often and history.counts is None:
             raise ValueError("frequency and presence need a history that keeps counts")
         if once or often:
-            a.seen, a.history_rows = history.seen.data_ptr(), history.n_rows
+            a.seen, a.history_rows = _address(history.seen, "seen"), history.n_rows
         if often:
-            a.counts = history.counts.data_ptr()
+            a.counts = _address(history.counts, "counts")
     if bias is not None:
         a.bias, a.bias_stride = _row_array(bias, "bias", torch.float32, n, width, dev)
     if allowed is not None:
@@ -436,7 +447,7 @@ def _output(logits, out, out_dtype):
 
 
 def _forward(a, dev: int, out):
-    _call(_cabi.lib().dnatok_process_logits, dev, a, out.data_ptr(), _TYPES[out.dtype], out.stride(0))
+    _call(_cabi.lib().dnatok_process_logits, dev, a, _address(out, "out"), _TYPES[out.dtype], out.stride(0))
     return out
 
 
@@ -445,6 +456,7 @@ def _backward(a, dev: int, dtype, grad, bias_shape, want_logits: bool):
     if grad.shape[1] > 1 and grad.stride(1) != 1:
         grad = grad.contiguous()
     n, width = grad.shape
+    d_grad = _address(grad, "grad")
     L = _cabi.lib()
     dx = grad.new_empty((n, width), dtype=dtype) if want_logits else None
     db, scratch, need = None, None, 0
@@ -455,7 +467,7 @@ def _backward(a, dev: int, dtype, grad, bias_shape, want_logits: bool):
             need = L.dnatok_logits_scratch_bytes(n, width)
             if need:
                 scratch = grad.new_empty((need,), dtype=torch.uint8)
-    _call(L.dnatok_process_logits_backward, dev, a, grad.data_ptr(), _TYPES[grad.dtype], grad.stride(0),
+    _call(L.dnatok_process_logits_backward, dev, a, d_grad, _TYPES[grad.dtype], grad.stride(0),
           dx.data_ptr() if dx is not None else None, width, db.data_ptr() if db is not None else None,
           scratch.data_ptr() if need else None, need)
     return dx, db
@@ -485,16 +497,16 @@ class _Process(torch.autograd.Function):
         a.dtype, a.repetition = _TYPES[ctx.dtype], ctx.number
         a.n_rows, a.width = grad.shape
         if logits is None:
-            a.logits = grad.data_ptr()               # not read: no token counts as seen
+            a.logits = _address(grad, "grad")        # not read: no token counts as seen
         else:
-            a.logits, a.stride = logits.data_ptr(), logits.stride(0)
-            a.seen, a.history_rows = seen.data_ptr(), seen.shape[0]
+            a.logits, a.stride = _address(logits, "logits"), logits.stride(0)
+            a.seen, a.history_rows = _address(seen, "seen"), seen.shape[0]
             if rows is not None:
-                a.rows, a.rows_bits = rows.data_ptr(), _BITS[rows.dtype]
+                a.rows, a.rows_bits = _address(rows, "rows"), _BITS[rows.dtype]
             if repetition is not None:
-                a.d_repetition = repetition.data_ptr()
+                a.d_repetition = _address(repetition, "repetition")
         if allowed is not None:
-            a.allowed, a.allowed_stride = allowed.data_ptr(), 0 if _shared(allowed.shape) else allowed.stride(0)
+            a.allowed, a.allowed_stride = _address(allowed, "allowed"), 0 if _shared(allowed.shape) else allowed.stride(0)
         dx, db = _backward(a, grad.get_device(), ctx.dtype, grad, ctx.bias_shape if ctx.needs_input_grad[1] else None, ctx.needs_input_grad[0])
         return dx, db, None, None, None, None, None, None, None
 

@@ -137,3 +137,45 @@ def test_a_bias_alone_keeps_no_logits(library):  # noqa: F811
     h.append(torch.zeros(3, dtype=torch.int64))
     db, = torch.autograd.grad(y, b, torch.ones(3, 40))
     assert db.shape == (40,) and library.calls[-1][1].seen is None
+
+
+def wrapper(t):
+    """A tensor that stands for others and has no memory of its own, as torch's distributed ones."""
+    class Wrapper(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError("no operation of it is expected: %s" % func)
+    return torch.Tensor._make_wrapper_subclass(Wrapper, t.shape, strides=t.stride(), dtype=t.dtype, device=t.device)
+
+
+@pytest.mark.parametrize("name", ["logits", "bias", "allowed", "repetition", "frequency", "presence", "rows", "out", "seen", "counts"])
+def test_tensors_without_memory_are_refused(library, name):  # noqa: F811
+    """An address of 0 means an argument that is not there."""
+    h = history(3, 40)
+    args = dict(logits=torch.randn(3, 40), bias=torch.randn(40), allowed=torch.zeros((3, 2), dtype=torch.int32), repetition=torch.ones(3), frequency=torch.ones(3),
+                presence=torch.ones(3), rows=torch.zeros(3, dtype=torch.int64), out=torch.empty(3, 40))
+    process_logits(history=h, **args)
+    library.calls.clear()
+    if name in args:
+        args[name] = wrapper(args[name])
+    else:
+        setattr(h, name, wrapper(getattr(h, name)))
+    with pytest.raises(ValueError, match="%s has no memory" % name):
+        process_logits(history=h, **args)
+    assert not library.calls
+
+
+def test_histories_and_grammars_refuse_tensors_without_memory(library):  # noqa: F811
+    h, g = history(3, 40), Grammar(Automaton.avoiding(["ACG"]), [b"A", b"C"] * 20)
+    library.calls.clear()
+    ids, n, t = torch.zeros((3, 5), dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int64)
+    offsets = torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: h.add(wrapper(ids)), lambda: h.add(ids, wrapper(n)), lambda: h.add(t, offsets=wrapper(offsets)), lambda: h.append(wrapper(t)),
+                 lambda: h.append(t, rows=wrapper(t)), lambda: g.allowed(wrapper(n)), lambda: g.allowed(n, out=wrapper(torch.zeros((3, 2), dtype=torch.int32))),
+                 lambda: g.advance(n, wrapper(t)), lambda: g.advance(n, t, out=wrapper(n)), lambda: g.step(n, t, out_allowed=wrapper(torch.zeros((3, 2), dtype=torch.int32))),
+                 lambda: process_logits_backward(wrapper(torch.zeros(3, 40)), torch.zeros(3, 40))):
+        with pytest.raises(ValueError, match="has no memory"):
+            call()
+    assert not library.calls
+    empty = torch.zeros((0, 40))
+    process_logits(empty, bias=torch.zeros((0, 40)), allowed=torch.zeros((0, 2), dtype=torch.int32))
