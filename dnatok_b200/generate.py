@@ -138,16 +138,21 @@ class TokenHistory:
         device = torch.device("cuda" if device is None else device if not isinstance(device, int) else "cuda:%d" % device)
         if device.type != "cuda":
             raise RuntimeError("a history is kept in CUDA tensors; there is no CPU path")
-        words = _words(width)
         self.n_rows, self.width = n_rows, width
         self.counts: Optional[torch.Tensor] = None
-        if counts:                                   # one array, cleared at once: the words, then the counts
-            split = (n_rows * words + 3) // 4 * 4
-            both = torch.zeros(split + n_rows * width, dtype=torch.int32, device=device)
-            self.seen = both.as_strided((n_rows, words), (words, 1))
-            self.counts = both.as_strided((n_rows, width), (width, 1), split)
+        if counts:
+            self.seen, self.counts = self._cleared(n_rows, width, device)
         else:
-            self.seen = torch.zeros((n_rows, words), dtype=torch.int32, device=device)
+            self.seen = torch.zeros((n_rows, _words(width)), dtype=torch.int32, device=device)
+
+    @staticmethod
+    def _cleared(n_rows: int, width: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(seen, counts) in one array, cleared at once: the words, then the counts."""
+        words = _words(width)
+        split = (n_rows * words + 3) // 4 * 4
+        both = torch.zeros(split + n_rows * width, dtype=torch.int32, device=device)
+        # (.data: views of one array would share its version, and a write to the counts would count as one to the words)
+        return both.as_strided((n_rows, words), (words, 1)).data, both.as_strided((n_rows, width), (width, 1), split).data
 
     @property
     def device(self) -> torch.device:

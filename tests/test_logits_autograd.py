@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from dnatok_b200 import Automaton, Grammar, process_logits, process_logits_backward  # noqa: E402
+from dnatok_b200 import Automaton, Grammar, TokenHistory, process_logits, process_logits_backward  # noqa: E402
 
 from generate_host import history, library  # noqa: E402,F401
 
@@ -179,3 +179,37 @@ def test_histories_and_grammars_refuse_tensors_without_memory(library):  # noqa:
     assert not library.calls
     empty = torch.zeros((0, 40))
     process_logits(empty, bias=torch.zeros((0, 40)), allowed=torch.zeros((0, 2), dtype=torch.int32))
+
+
+def test_counts_and_seen_change_by_themselves(library):  # noqa: F811
+    """The backward pass reads what was seen: counts that are cleared in between do not matter to it, marks do."""
+    seen, counts = TokenHistory._cleared(3, 40, torch.device("cpu"))
+    assert seen.shape == (3, 2) and counts.shape == (3, 40) and seen.is_contiguous() and counts.is_contiguous()
+    assert seen.dtype == counts.dtype == torch.int32 and not seen.any() and not counts.any()
+    assert counts.untyped_storage().data_ptr() == seen.untyped_storage().data_ptr() and counts.data_ptr() - seen.data_ptr() == 32
+    h = history(3, 40)
+    for write, refused in ((lambda: h.counts.zero_(), False), (lambda: h.seen.zero_(), True)):
+        h.seen, h.counts = TokenHistory._cleared(3, 40, torch.device("cpu"))
+        x = torch.randn(3, 40, requires_grad=True)
+        y = process_logits(x, history=h, repetition=1.5, frequency=0.5)
+        write()
+        if refused:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.sum().backward()
+        else:
+            y.sum().backward()
+            assert x.grad.shape == x.shape
+    with torch.inference_mode():
+        seen, counts = TokenHistory._cleared(0, 40, torch.device("cpu"))
+    assert seen.shape == (0, 2) and counts.shape == (0, 40)
+
+
+@pytest.mark.gpu
+def test_counts_may_be_cleared_before_the_backward_pass():
+    x, g = torch.randn(5, 700, device="cuda", requires_grad=True), torch.randn(5, 700, device="cuda")
+    h = TokenHistory(5, 700)
+    h.add(torch.randint(0, 700, (5, 300), device="cuda"), generated=True)
+    want, = torch.autograd.grad(process_logits(x, history=h, repetition=1.5, frequency=0.5), x, g)
+    y = process_logits(x, history=h, repetition=1.5, frequency=0.5)
+    h.counts.zero_()
+    assert torch.equal(torch.autograd.grad(y, x, g)[0], want) and not torch.equal(want, g)
