@@ -97,6 +97,56 @@ int check_output(const char* what, const void* p, size_t size, int64_t stride, c
     return 0;
 }
 
+// Rows of an array, all in bytes.  (128 bits: no stride is too long.)
+using Wide = __int128;
+struct Rows {
+    const void* p;
+    Wide n, stride, row;
+};
+
+// Whether two arrays have a byte in common.  Rows may lie between those of the other array, as the columns of a view of one
+// wider array do.
+bool overlap(Rows a, Rows b) {
+    if (!a.p || !b.p || a.n < 1 || b.n < 1 || a.row < 1 || b.row < 1) return false;
+    if (a.stride == 0) a.n = 1;
+    if (b.stride == 0) b.n = 1;
+    const Wide a0 = (Wide)(uintptr_t)a.p, b0 = (Wide)(uintptr_t)b.p;
+    const Wide a1 = a0 + (a.n - 1) * a.stride + a.row, b1 = b0 + (b.n - 1) * b.stride + b.row;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (a.n > 1 && b.n > 1 && a.stride == b.stride) {
+        // row j of b is b0 - a0 + (j - i) stride behind row i of a: the first such distance that does not end before a's row
+        const Wide d = b0 - a0, from = -b.row - d, s = a.stride;
+        Wide m = (from >= 0 ? from / s : -((-from + s - 1) / s)) + 1;
+        if (m < 1 - a.n) m = 1 - a.n;
+        return m <= b.n - 1 && d + m * s < a.row;
+    }
+    for (Wide i = 0, j = 0; i < a.n && j < b.n;) {             // both in order: the row that ends first is passed
+        const Wide x = a0 + i * a.stride, y = b0 + j * b.stride;
+        if (x + a.row <= y) i += a.n == 1 ? 1 : (y - x - a.row) / a.stride + 1;
+        else if (y + b.row <= x) j += b.n == 1 ? 1 : (x - y - b.row) / b.stride + 1;
+        else return true;
+    }
+    return false;
+}
+
+// An output may not overlap what other threads still read.  The logits themselves are the caller's to look at.
+int check_apart(const char* what, const Rows& out, const dnatok_logits* in) {
+    const Wide n = in->n_rows, width = in->width, words = (width + 31) / 32;
+    const struct { const char* name; Rows rows; } read[] = {
+        {"bias", {in->bias, n, (Wide)in->bias_stride * 4, width * 4}},
+        {"mask", {in->allowed, n, (Wide)in->allowed_stride * 4, words * 4}},
+        {"history's words", {in->seen, in->history_rows, words * 4, words * 4}},
+        {"history's counts", {in->counts, in->history_rows, width * 4, width * 4}},
+        {"row numbers", {in->seen ? in->rows : nullptr, n, in->rows_bits / 8, in->rows_bits / 8}},
+        {"repetition penalties", {in->d_repetition, n, 4, 4}},
+        {"frequency penalties", {in->d_frequency, n, 4, 4}},
+        {"presence penalties", {in->d_presence, n, 4, 4}},
+    };
+    for (const auto& r : read)
+        if (overlap(out, r.rows)) return abi_fail(DNATOK_ERR_INVALID, "%s and %s overlap", what, r.name);
+    return 0;
+}
+
 // Whether rows of elements of `size` bytes can be moved 16 bytes at a time.  An array that is not there can.
 bool vector_rows(const void* p, int64_t stride, size_t size, int64_t n_rows) {
     return !p || (aligned(p, 16) && (n_rows <= 1 || stride * (int64_t)size % 16 == 0));
@@ -160,6 +210,11 @@ int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtyp
     if (d_out == in->logits && in->n_rows && (out_dtype != in->dtype || (in->n_rows > 1 && out_stride != in->stride)))
         return abi_fail(DNATOK_ERR_INVALID, "in place the output has the logits' type and stride");
     if (in->n_rows == 0) return DNATOK_OK;
+    const Wide size = size_of(in->dtype), out_size = size_of(out_dtype);
+    const Rows out = {d_out, in->n_rows, out_stride * out_size, in->width * out_size};
+    if (d_out != in->logits && overlap(out, {in->logits, in->n_rows, in->stride * size, in->width * size}))
+        return abi_fail(DNATOK_ERR_INVALID, "output and logits overlap (the output may be the logits themselves)");
+    if (int rc = check_apart("output", out, in)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     const LogitsArgs a = logits_args(in);
     const bool vector = vector_rows(in->logits, in->stride, size_of(in->dtype), in->n_rows) &&

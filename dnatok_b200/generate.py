@@ -519,7 +519,8 @@ class _Process(torch.autograd.Function):
 def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None, repetition: Number = 1.0,
                    frequency: Number = 0.0, presence: Number = 0.0, bias=None, allowed=None, out=None, out_dtype=None):
     """``logits`` [n, width] (float32, float16 or bfloat16; a view such as ``model_output[:, -1]`` is fine) after penalties,
-    bias and mask, as a new tensor of its type or of ``out_dtype`` float32, or in ``out`` (which may be ``logits``).
+    bias and mask, as a new tensor of its type or of ``out_dtype`` float32, or in ``out``, which may be ``logits`` but may
+    not overlap them, or another argument, in any other way.
 
     * A token the row has seen: ``x > 0 ? x / repetition : x * repetition``; one it generated ``c > 0`` times, then
       ``- frequency * c - presence``.  Each is a number, or a float32 tensor [n] (repetition from 2^-126 to 2^126 there too).

@@ -314,7 +314,7 @@ typedef struct {
  * keep x.  Computed in 32 bits,
  * rounded once to the output's type: that of the logits or DNATOK_F32.  Logits that are not allowed have no influence, NaN
  * included; a row without an allowed token is -inf throughout.  d_out may be the logits themselves (same type and stride);
- * another overlap is not allowed. */
+ * another overlap, with any array of the call, is refused. */
 int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtype, int64_t out_stride, dnatok_stream stream);
 
 /* Bytes of 256-byte aligned device scratch that dnatok_process_logits_backward needs for a shared bias' gradient. */
