@@ -286,6 +286,29 @@ int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, 
     if (join && (!d_scratch || scratch_bytes < dnatok_logits_scratch_bytes(a.n_rows, a.width) || !aligned(d_scratch, 256)))
         return abi_fail(DNATOK_ERR_SCRATCH, "the gradient of a shared bias needs %zu bytes of 256-byte aligned scratch",
                         dnatok_logits_scratch_bytes(a.n_rows, a.width));
+    dnatok_logits read = *in;                                 // what the kernels read of it
+    read.bias = read.d_frequency = read.d_presence = nullptr;
+    read.counts = nullptr;
+    if (!in->seen || !d_dlogits) {
+        read.logits = read.rows = nullptr;
+        read.seen = nullptr;
+        read.d_repetition = nullptr;
+    }
+    const Wide size = size_of(in->dtype), width = in->width;
+    const Rows grad = {d_grad, in->n_rows, grad_stride * (Wide)size_of(grad_dtype), width * size_of(grad_dtype)};
+    const Rows logits = {read.logits, in->n_rows, in->stride * size, width * size};
+    const Rows outs[] = {{d_dlogits, in->n_rows, dlogits_stride * size, width * size},
+                         {d_dbias, shared ? 1 : in->n_rows, width * 4, width * 4},
+                         {join ? d_scratch : nullptr, 1, 0, join ? (Wide)dnatok_logits_scratch_bytes(a.n_rows, a.width) : 0}};
+    const char* names[] = {"logits' gradient", "bias' gradient", "scratch"};
+    for (int i = 0; i < 3; ++i) {
+        if (overlap(outs[i], logits)) return abi_fail(DNATOK_ERR_INVALID, "%s and logits overlap", names[i]);
+        if (!(i == 0 && d_dlogits == d_grad) && overlap(outs[i], grad))
+            return abi_fail(DNATOK_ERR_INVALID, "%s and gradient overlap (that of the logits may be the gradient itself)", names[i]);
+        for (int k = 0; k < i; ++k)
+            if (overlap(outs[i], outs[k])) return abi_fail(DNATOK_ERR_INVALID, "%s and %s overlap", names[i], names[k]);
+        if (int rc = check_apart(names[i], outs[i], &read)) return rc;
+    }
     float* sums = join ? (float*)d_scratch : d_dbias;
     with_type(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;

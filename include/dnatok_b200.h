@@ -324,7 +324,7 @@ size_t dnatok_logits_scratch_bytes(int64_t n_rows, int64_t width);
  * logits' type; NULL: not wanted) and d_dbias (float, [width] where bias_stride is 0, else [n_rows, width] contiguous;
  * NULL: not wanted).  in->bias and in->counts are not read.  A shared bias' gradient is summed in 32 bits in an order
  * that depends on the sizes only.  d_dlogits may be d_grad itself where type and stride are the same; it may
- * not be the logits. */
+ * not be the logits, and another overlap of what is written with what is read or written is refused. */
 int dnatok_process_logits_backward(const dnatok_logits* in, const void* d_grad, int32_t grad_dtype, int64_t grad_stride,
                                    void* d_dlogits, int64_t dlogits_stride, float* d_dbias, void* d_scratch,
                                    size_t scratch_bytes, dnatok_stream stream);

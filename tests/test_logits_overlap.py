@@ -112,3 +112,45 @@ def test_views_of_one_array():
         process_logits(x, out=h.counts.view(torch.float32), **kw)
     assert torch.equal(x, before) and torch.equal(process_logits(x, **kw), want)
     assert torch.equal(process_logits(x, out=x, **kw), want)
+
+
+def backward(grad=2 * BASE, grad_stride=40, dlogits=4 * BASE, dlogits_stride=40, dbias=6 * BASE, scratch=None, scratch_bytes=0, **kw):
+    a = _cabi.Logits(logits=16 * BASE, dtype=0, n_rows=3, width=40, stride=40, seen=32 * BASE, history_rows=3, allowed=48 * BASE, allowed_stride=2, repetition=1.0)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return refused(_cabi.lib().dnatok_process_logits_backward(ctypes.byref(a), grad, 0, grad_stride, dlogits, dlogits_stride, dbias, scratch, scratch_bytes, None))
+
+
+def test_gradients_over_what_the_call_reads(no_gpu):
+    at = 8 * BASE
+    assert not backward()
+    assert not backward(grad=at, dlogits=at)                       # in place
+    assert not backward(grad=at, dlogits=at + 160, grad_stride=80, dlogits_stride=80)
+    assert backward(grad=at, dlogits=at + 156, grad_stride=80, dlogits_stride=80)
+    for move in (-476, -4, 4, 476):
+        assert backward(grad=at, dlogits=at + move)
+        assert backward(logits=at, dlogits=at + move)
+        assert backward(grad=at, dlogits=at + move, seen=None)
+        assert not backward(logits=at, dlogits=at + move, seen=None)           # these are not read then
+        assert not backward(logits=at, dbias=at, dlogits=None)
+        assert backward(dbias=at, dlogits=at + move, bias_stride=40)
+    for out in ("dlogits", "dbias"):
+        for name, kw, bytes_ in [("allowed", {}, 24), ("seen", {}, 24), ("rows", dict(rows_bits=64, history_rows=3), 24), ("d_repetition", {}, 12)]:
+            for here, want in [(at, True), (at + bytes_ - 4, True), (at + bytes_, False)]:
+                assert backward(**{name: at, out: here}, **kw) == want
+        for name in ("bias", "counts", "d_frequency", "d_presence"):           # not read
+            assert not backward(**{name: at, out: at}, bias_stride=0)
+    assert backward(grad=at, dbias=at) and backward(grad=at, dbias=at + 476) and not backward(grad=at, dbias=at + 480)
+    assert backward(logits=at, dbias=at + 476) and backward(dlogits=at, dbias=at + 476) and not backward(dlogits=at, dbias=at + 480)
+
+
+def test_scratch_over_what_the_call_reads_or_writes(no_gpu):
+    n, width, at = 1000, 40, 8 * BASE
+    need = _cabi.lib().dnatok_logits_scratch_bytes(n, width)
+    assert need > 1024
+    good = dict(n_rows=n, history_rows=n, scratch=at, scratch_bytes=need + 10 ** 6)
+    assert not backward(**good)
+    for name, bytes_ in [("grad", n * 160), ("dlogits", n * 160), ("dbias", 160), ("logits", n * 160), ("allowed", n * 8), ("seen", n * 8), ("d_repetition", n * 4)]:
+        end = at + (need + 7 & ~7)
+        for here, want in [(at, True), (at + need - 4 & ~3, True), (end, False), (at - bytes_ + 4, True), (at - bytes_, False)]:
+            assert backward(**{**good, name: here}) == want, (name, here - at)
