@@ -495,6 +495,9 @@ int grammar_tables(dnatok_grammar* g, cudaStream_t stream, GrammarTables* out) {
     return 0;
 }
 
+Rows row_array(const void* p, int64_t n_rows, Wide row) { return {p, n_rows, row, row}; }
+Wide mask_bytes(const dnatok_grammar* g) { return (Wide)((g->width + 31) / 32) * 4; }
+
 int check_states(const dnatok_grammar* g, const void* states, int64_t n_rows) {
     if (!g || n_rows < 0 || (n_rows && !states)) return abi_fail(DNATOK_ERR_INVALID, "bad argument");
     if (!aligned(states, 4)) return abi_fail(DNATOK_ERR_INVALID, "misaligned states");
@@ -703,6 +706,7 @@ int dnatok_grammar_allowed(dnatok_grammar* g, const int32_t* d_states, int64_t n
     if (n_rows && !d_allowed) return abi_fail(DNATOK_ERR_INVALID, "mask is NULL");
     if (!aligned(d_allowed, 4)) return abi_fail(DNATOK_ERR_INVALID, "misaligned mask");
     if (n_rows == 0) return DNATOK_OK;
+    if (overlap(row_array(d_allowed, n_rows, mask_bytes(g)), row_array(d_states, n_rows, 4))) return abi_fail(DNATOK_ERR_INVALID, "mask and states overlap");
     GrammarTables t;
     if (int rc = grammar_tables(g, (cudaStream_t)stream, &t)) return rc;
     return launch_allowed(t, d_states, nullptr, 0, nullptr, n_rows, d_allowed, (cudaStream_t)stream);
@@ -717,6 +721,14 @@ int dnatok_grammar_step(dnatok_grammar* g, const int32_t* d_states, const void* 
         return abi_fail(DNATOK_ERR_INVALID, "misaligned array");
     if (d_allowed && d_states_out == d_states && n_rows) return abi_fail(DNATOK_ERR_INVALID, "with a mask the new states need an array of their own");
     if (n_rows == 0) return DNATOK_OK;
+    // With a mask every block of a row reads its state and token while the first writes the new state.  Without one a thread has
+    // a row, and may write where it read.
+    const Rows states = row_array(d_states, n_rows, 4), tokens = row_array(d_tokens, n_rows, token_bits / 8), out = row_array(d_states_out, n_rows, 4);
+    if (d_states_out != d_states && overlap(out, states)) return abi_fail(DNATOK_ERR_INVALID, "new states and states overlap");
+    if ((d_allowed || token_bits != 32 || d_states_out != d_tokens) && overlap(out, tokens))
+        return abi_fail(DNATOK_ERR_INVALID, "new states and tokens overlap");
+    const Rows mask = row_array(d_allowed, n_rows, mask_bytes(g));
+    if (overlap(mask, states) || overlap(mask, tokens) || overlap(mask, out)) return abi_fail(DNATOK_ERR_INVALID, "mask and states or tokens overlap");
     GrammarTables t;
     cudaStream_t st = (cudaStream_t)stream;
     if (int rc = grammar_tables(g, st, &t)) return rc;

@@ -88,8 +88,8 @@ __device__ __forceinline__ int64_t grammar_token(const void* tokens, int token_b
 }
 
 __global__ void __launch_bounds__(GRAMMAR_THREADS)
-grammar_advance_kernel(GrammarTables t, const int32_t* states, const void* __restrict__ tokens, int token_bits, int64_t n_rows,
-                       int32_t* out) {
+grammar_advance_kernel(GrammarTables t, const int32_t* states, const void* tokens, int token_bits, int64_t n_rows,
+                       int32_t* out) {                        // (out may be the states, or the tokens)
     const int64_t row = (int64_t)blockIdx.x * GRAMMAR_THREADS + threadIdx.x;
     if (row < n_rows) out[row] = grammar_after(t, states[row], grammar_token(tokens, token_bits, row));
 }

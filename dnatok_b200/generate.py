@@ -323,7 +323,7 @@ class Grammar:
 
     def advance(self, states, tokens, *, out=None) -> torch.Tensor:
         """int32 [n]: the states after ``tokens`` [n] (int32 or int64); a token outside the vocabulary (-1, say) leaves its
-        row as it was.  ``out`` may be ``states``."""
+        row as it was.  ``out`` may be ``states``, but may not overlap them in another way."""
         n, dev, at = self._states(states)
         bits = _tokens(tokens, "tokens", n, dev)
         new = self._new_states(states, n, dev, out)
@@ -334,7 +334,8 @@ class Grammar:
         return new
 
     def step(self, states, tokens, *, out=None, out_allowed=None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """``advance`` and the masks of the new states in one call: (states, allowed).  ``out`` may not be ``states``."""
+        """``advance`` and the masks of the new states in one call: (states, allowed).  ``out`` may not overlap ``states``
+        or ``tokens``, nor ``out_allowed`` any of them."""
         n, dev, at = self._states(states)
         bits = _tokens(tokens, "tokens", n, dev)
         new = self._new_states(states, n, dev, out)

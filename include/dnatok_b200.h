@@ -367,7 +367,8 @@ int dnatok_grammar_allowed(dnatok_grammar* g, const int32_t* d_states, int64_t n
                            dnatok_stream stream);
 
 /* d_states_out[row] = the state after d_tokens[row] (token_bits 32 or 64); a token outside [0, width) leaves the row as it
- * was.  With d_allowed, the masks of the new states too; d_states_out may then not be d_states. */
+ * was.  With d_allowed, the masks of the new states too.  Without, d_states_out may be d_states, or d_tokens of 32 bits; another
+ * overlap of an output with an input, and any with d_allowed, is refused. */
 int dnatok_grammar_step(dnatok_grammar* g, const int32_t* d_states, const void* d_tokens, int32_t token_bits, int64_t n_rows,
                         int32_t* d_states_out, uint32_t* d_allowed, dnatok_stream stream);
 
