@@ -28,15 +28,28 @@ def base_classes(lowercase: bool = True) -> np.ndarray:
     return table
 
 
+def whole_numbers(values, dtype, what: str) -> np.ndarray:
+    """A contiguous array of ``dtype`` with these values; one that the type does not hold is refused, not wrapped or cut."""
+    given = np.asarray(values)
+    try:
+        with np.errstate(invalid="ignore"):
+            a = np.ascontiguousarray(given, dtype=dtype)
+    except (OverflowError, TypeError, ValueError):
+        a = None
+    if a is None or not np.array_equal(a, given):
+        raise ValueError("%s must hold whole numbers of %s" % (what, np.dtype(dtype).name))
+    return a
+
+
 class Automaton:
     """``next_state`` int [states, classes] (-1: no way on), ``accepting`` [states], ``byte_class`` uint8[256] (which column
     a byte takes; bases and others by default), ``start`` the first state.  From every state the row may go on as long as
     a token leads to a state; the end token is allowed in accepting states."""
 
     def __init__(self, next_state, accepting, *, byte_class=None, start: int = 0):
-        self.next_state = np.ascontiguousarray(next_state, dtype=np.int32)
-        self.accepting = np.ascontiguousarray(accepting, dtype=np.uint8)
-        self.byte_class = np.ascontiguousarray(base_classes() if byte_class is None else byte_class, dtype=np.uint8)
+        self.next_state = whole_numbers(next_state, np.int32, "next_state")
+        self.accepting = np.ascontiguousarray(np.asarray(accepting) != 0, dtype=np.uint8)
+        self.byte_class = whole_numbers(base_classes() if byte_class is None else byte_class, np.uint8, "byte_class")
         if self.next_state.ndim != 2 or not self.next_state.shape[0] or not self.next_state.shape[1]:
             raise ValueError("next_state must be [states, classes]")
         n, classes = self.next_state.shape

@@ -36,7 +36,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _cabi
-from .automaton import Automaton
+from .automaton import Automaton, whole_numbers
 
 DEAD, FINISHED = _cabi.STATE_DEAD, _cabi.STATE_FINISHED
 _TYPES = {torch.float32: _cabi.F32, torch.float16: _cabi.F16, torch.bfloat16: _cabi.BF16}
@@ -245,8 +245,8 @@ class Grammar:
     def __init__(self, automaton: Automaton, tokens: Union[Sequence[Optional[bytes]], Tuple[np.ndarray, np.ndarray]], *,
                  end_id: Optional[int] = None, width: Optional[int] = None):
         if isinstance(tokens, tuple) and len(tokens) == 2 and isinstance(tokens[0], np.ndarray):
-            flat = np.ascontiguousarray(tokens[0], dtype=np.uint8).reshape(-1)
-            offsets = np.ascontiguousarray(tokens[1], dtype=np.int64)
+            flat = whole_numbers(tokens[0], np.uint8, "token bytes").reshape(-1)
+            offsets = whole_numbers(tokens[1], np.int64, "token offsets")
         else:
             tokens = [bytes(t or b"") for t in tokens]
             flat = np.frombuffer(b"".join(tokens), dtype=np.uint8)
