@@ -248,6 +248,10 @@ class Grammar:
             flat = whole_numbers(tokens[0], np.uint8, "token bytes").reshape(-1)
             offsets = whole_numbers(tokens[1], np.int64, "token offsets")
         else:
+            tokens = list(tokens)
+            for v, t in enumerate(tokens):
+                if isinstance(t, (int, np.generic)):               # (bytes(5) would be five zeros)
+                    raise TypeError("token %d is a number; a token is its bytes, or None" % v)
             tokens = [bytes(t or b"") for t in tokens]
             flat = np.frombuffer(b"".join(tokens), dtype=np.uint8)
             offsets = np.zeros(len(tokens) + 1, dtype=np.int64)

@@ -41,3 +41,14 @@ def test_token_bytes_that_are_none():
             Grammar(a, (flat, np.array(offsets)))
     for flat in (np.array([65, 66]), np.array([65, 66], np.int8), np.array([65.0, 66.0])):
         Grammar(a, (flat, np.array([0, 1, 2], np.int32))).close()
+
+
+def test_ids_in_place_of_bytes():
+    """A number is no text: bytes(5) would be five zeros."""
+    a = Automaton(NEXT, [1, 1])
+    for tokens in ([b"A", 5], [0, 1, 2], [np.int64(3)], [True]):
+        with pytest.raises(TypeError, match="token"):
+            Grammar(a, tokens)
+    g = Grammar(a, [b"A", bytearray(b"CG"), None, b"", memoryview(b"T"), [65, 67]])
+    assert g.width == 6
+    g.close()
