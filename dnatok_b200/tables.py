@@ -39,6 +39,8 @@ class Specials:
     cls_id: int = -1          # id emitted before the sequence when add_special_tokens, -1: none
     sep_id: int = -1          # id emitted after the sequence, -1: none
     padding_side: str = "right"
+    pad_named: bool = True    # False: the tokenizer names no pad id, and pad_id is a stand-in that may be an ordinary token
+    unk_named: bool = True
 
 
 @dataclass
@@ -232,10 +234,11 @@ def bpe_spec_from_json(cfg: Dict[str, Any], *, pad_id: Optional[int] = None,
         if len(c) == 1 and ord(c) < 128:
             raise UnsupportedTokenizer("single-character added token %r" % c)
     cls_id, sep_id = _template_specials(cfg)
+    pad_named = pad_id is not None or "[PAD]" in vocab or "<pad>" in vocab
     if pad_id is None:
         pad_id = vocab.get("[PAD]", vocab.get("<pad>", 0))
     vs = max(max(vocab.values()) + 1, max((t["id"] for t in cfg.get("added_tokens", [])), default=-1) + 1)
-    return TokenizerSpec("bpe", Specials(pad_id, unk_id, cls_id, sep_id, padding_side), vs, lut,
+    return TokenizerSpec("bpe", Specials(pad_id, unk_id, cls_id, sep_id, padding_side, pad_named), vs, lut,
                          merge_a=a, merge_b=b, merge_out=o, normalizer=compile_normalizer(cfg),
                          vocab=dict(vocab))
 
@@ -297,8 +300,10 @@ def detect_kmer(tok: Any) -> int:
 
 def spec_from_probing(tok: Any) -> TokenizerSpec:
     """Char or k-mer tables by asking the tokenizer, as the reference's discovery does."""
-    pad_id = int(getattr(tok, "pad_token_id", 0) or 0)
+    pad_id = getattr(tok, "pad_token_id", None)
     unk_id = getattr(tok, "unk_token_id", None)
+    pad_named, unk_named = pad_id is not None, unk_id is not None
+    pad_id = int(pad_id or 0)
     unk_id = int(unk_id) if unk_id is not None else 0
     side = getattr(tok, "padding_side", "right")
     cls_id, sep_id = _probe_specials(tok)
@@ -307,7 +312,7 @@ def spec_from_probing(tok: Any) -> TokenizerSpec:
     except Exception:
         vocab = {}
     vs = max(int(getattr(tok, "vocab_size", 0) or 0), (max(vocab.values()) + 1) if vocab else 0)
-    sp = Specials(pad_id, unk_id, cls_id, sep_id, side)
+    sp = Specials(pad_id, unk_id, cls_id, sep_id, side, pad_named, unk_named)
 
     singles = np.full(256, unk_id, np.int32)
     chars = [c for c in range(1, 128) if not chr(c).isspace()]
@@ -460,9 +465,10 @@ def spec_from_tokenizer(tok: Any) -> TokenizerSpec:
 
 def token_bytes(spec: TokenizerSpec) -> List[bytes]:
     """The text every id stands for (empty: a special, the unknown id or an id without one), from the tables the kernels
-    encode with.  Where several bytes give one id (soft-masked letters, say) it is the upper-case one."""
+    encode with.  Where several bytes give one id (soft-masked letters, say) it is the upper-case one.  A pad or unknown
+    id that the tokenizer does not name is no special."""
     sp = spec.specials
-    special = {sp.pad_id, sp.unk_id, sp.cls_id, sp.sep_id}
+    special = {sp.cls_id, sp.sep_id} | ({sp.pad_id} if sp.pad_named else set()) | ({sp.unk_id} if sp.unk_named else set())
     luts = [np.asarray(spec.lut256)] + ([np.asarray(spec.start_lut256)] if spec.start_lut256 is not None else [])
     tops = [int(a.max()) for a in luts + [np.asarray(x) for x in (spec.kmer_ids, spec.kmer_table5, spec.merge_out) if x is not None and len(x)]]
     text = [b""] * max([spec.vocab_size] + [t + 1 for t in tops])
@@ -471,7 +477,7 @@ def token_bytes(spec: TokenizerSpec) -> List[bytes]:
         if i >= 0 and i not in special and not text[i]:
             text[i] = b
 
-    upper_first = sorted(range(256), key=lambda c: (not 65 <= c <= 90, c))
+    upper_first = sorted(range(256), key=lambda c: (not 65 <= c <= 90, not 33 <= c <= 126, c))
     for lut in luts:
         for c in upper_first:
             put(int(lut[c]), bytes([c]))
