@@ -506,3 +506,14 @@ def token_bytes(spec: TokenizerSpec) -> List[bytes]:
                 break
             left = wait
     return text
+
+
+def following_bytes(spec: TokenizerSpec, *, first: bool = False) -> List[bytes]:
+    """``token_bytes`` without the ids that only begin a row, or, for its ``first`` token, without those that only follow one
+    (a character may have one id at the start of a row and another behind it)."""
+    text = token_bytes(spec)
+    if spec.start_lut256 is not None:
+        starts, others = set(np.asarray(spec.start_lut256).tolist()), set(np.asarray(spec.lut256).tolist())
+        for i in (others - starts if first else starts - others):
+            text[i] = b""
+    return text

@@ -314,13 +314,15 @@ class B200Tokenizer:
             raise ValueError("width %d is smaller than the vocabulary (%d tokens)" % (width, self.vocab_size))
         return TokenHistory(n_rows, width, device=self.device, counts=counts)
 
-    def grammar(self, automaton, *, width: Optional[int] = None):
+    def grammar(self, automaton, *, width: Optional[int] = None, first: bool = False):
         """A ``Grammar``: what the automaton allows of this vocabulary.  The separator ends a row; other specials and the
-        unknown token never follow."""
+        unknown token never follow.  Where a character has an id of its own at the start of a row, that id does not follow
+        either; ``first``: the grammar of a row's first token, which allows such ids and not those that only follow (states
+        are the automaton's in both)."""
         from .generate import Grammar
-        from .tables import token_bytes
+        from .tables import following_bytes
         sep = self.spec.specials.sep_id
-        return Grammar(automaton, token_bytes(self.spec), end_id=sep if sep >= 0 else None, width=width)
+        return Grammar(automaton, following_bytes(self.spec, first=first), end_id=sep if sep >= 0 else None, width=width)
 
     def _raise_on_status(self, status, truncation: bool) -> None:
         bits = int(status.max().item()) if status.numel() else 0

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from dnatok_b200 import Automaton
-from dnatok_b200.tables import bpe_spec_from_json, spec_from_tokenizer, token_bytes
+from dnatok_b200.tables import bpe_spec_from_json, following_bytes, spec_from_tokenizer, token_bytes
 
 
 class Letters:
@@ -47,3 +47,53 @@ def test_merges_without_a_pad_id(pad):
     text = token_bytes(bpe_spec_from_json(cfg, pad_id=pad))
     assert text[1:5] == [b"C", b"G", b"T", b""]
     assert (text[0], text[5], text[6]) == ((b"", b"", b"") if pad == 0 else (b"A", b"AC", b"ACG"))
+
+
+FIRST = {"A": 10, "C": 11, "G": 12, "T": 13}
+
+
+def split_tokenizer():
+    """Ids 10 .. 13 at the start of a text, 5 .. 8 behind it, N (9) at both; 3 ends a row."""
+    return Letters({"A": 5, "C": 6, "G": 7, "T": 8, "N": 9}, 9, first=FIRST, pad=0, unk=1, sep=3)
+
+
+def test_ids_of_the_start_and_of_what_follows():
+    s = spec_from_tokenizer(split_tokenizer())
+    assert s.start_lut256 is not None and s.specials.sep_id == 3
+    both = token_bytes(s)
+    assert [both[i] for i in (5, 6, 7, 8, 10, 11, 12, 13)] == [b"A", b"C", b"G", b"T"] * 2
+    follow, first = following_bytes(s), following_bytes(s, first=True)
+    assert len(follow) == len(first) == len(both)
+    for i in range(len(both)):
+        assert follow[i] == (b"" if i in FIRST.values() else both[i]) and first[i] == (b"" if i in (5, 6, 7, 8) else both[i])
+    plain = spec_from_tokenizer(Letters(BASES, 4))
+    assert following_bytes(plain) == following_bytes(plain, first=True) == token_bytes(plain)
+
+
+@pytest.mark.gpu
+def test_rows_never_start_again():
+    """A grammar's masks hold the ids that follow, those of a row's first token where asked for; states are the same."""
+    import torch
+    from dnatok_b200 import B200Tokenizer, process_logits
+    tok = B200Tokenizer(spec_from_tokenizer(split_tokenizer()))
+    automaton = Automaton.avoiding(["AA"])
+    first, follow = tok.grammar(automaton, first=True), tok.grammar(automaton)
+    bits = lambda words: {v for v in range(tok.vocab_size) if words.view(-1)[v // 32].item() >> (v % 32) & 1}  # noqa: E731
+    states = first.start(1)
+    assert bits(first.allowed(states)) == {3, 9, 10, 11, 12, 13} and bits(follow.allowed(states)) == {3, 5, 6, 7, 8, 9}
+    states, allowed = follow.step(first.advance(states, torch.tensor([10], device="cuda")), torch.tensor([-1], device="cuda"))
+    assert bits(allowed) == {3, 6, 7, 8, 9}                        # no A behind the A, and no start again
+    n, g = 32, torch.Generator(device="cuda").manual_seed(1)
+    states, rows = first.start(n), []
+    allowed = first.allowed(states)
+    for k in range(20):
+        tokens = process_logits(torch.randn((n, tok.vocab_size), generator=g, device="cuda"), allowed=allowed).argmax(-1)
+        rows.append(tokens.cpu().numpy())
+        states = (first if k == 0 else follow).advance(states, tokens)
+        allowed = follow.allowed(states)
+    assert (states != -1).all()
+    text = token_bytes(tok.spec)
+    for r in np.stack(rows, 1):
+        r = r[:list(r).index(3)] if 3 in r else r
+        word = b"".join(text[v] for v in r).decode()
+        assert "AA" not in word and r.tolist() == (split_tokenizer()([word])["input_ids"][0] if word else [])
