@@ -436,6 +436,14 @@ namespace {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
+// While it lives, calls of this thread that a capture does not allow leave the captures of other streams alone: allocations,
+// frees and waits that are no part of them.
+struct OutsideCaptures {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    bool on = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    ~OutsideCaptures() { if (on) cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // The tables on the current device, uploaded on first use: one allocation, filled on a stream of its own.
 int grammar_tables(dnatok_grammar* g, cudaStream_t stream, GrammarTables* out) {
     int dev = 0;
@@ -447,6 +455,7 @@ int grammar_tables(dnatok_grammar* g, cudaStream_t stream, GrammarTables* out) {
         CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
         if (capturing != cudaStreamCaptureStatusNone)
             return abi_fail(DNATOK_ERR_INVALID, "a grammar's first use on a device must be outside of stream capture");
+        OutsideCaptures outside;
         constexpr int N = 11;
         const size_t sizes[N] = {g->next.size() * 4, g->step16.size() * 2, g->accepting.size(), g->codes.size(), g->token_at.size() * 4,
                                  g->text.size() * 8, g->prefix.size() * 8, g->rest.size() * 8, g->step32.size() * 4, g->super.size() * 4, g->more.size() * 4};
@@ -688,14 +697,11 @@ int dnatok_create_grammar(const int32_t* next, int32_t n_states, int32_t n_class
 
 void dnatok_destroy_grammar(dnatok_grammar* g) {
     if (!g) return;
-    int cur = 0;
-    if (!g->dev.empty()) cudaGetDevice(&cur);
-    // may run while some stream is captured: a free is no part of the capture and must not end it
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    if (!g->dev.empty()) cudaThreadExchangeStreamCaptureMode(&mode);
-    for (auto& kv : g->dev) if (cudaSetDevice(kv.first) == cudaSuccess) cudaFree(kv.second.memory);
     if (!g->dev.empty()) {
-        cudaThreadExchangeStreamCaptureMode(&mode);
+        OutsideCaptures outside;                              // may run while some stream is captured
+        int cur = 0;
+        cudaGetDevice(&cur);
+        for (auto& kv : g->dev) if (cudaSetDevice(kv.first) == cudaSuccess) cudaFree(kv.second.memory);
         cudaSetDevice(cur);
     }
     delete g;

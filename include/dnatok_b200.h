@@ -282,7 +282,9 @@ int dnatok_set_option(const char* name, int64_t value);
  *
  * Sets of tokens are words of 32 bits, (width + 31) / 32 of them: bit v % 32 of word v / 32 stands for token v.  width is
  * the number of columns of the logits; it may exceed the vocabulary.  Device buffers are the caller's; a grammar owns
- * its tables (uploaded once per device on first use, which has to be outside of stream capture). */
+ * its tables.  They are uploaded on the grammar's first use on a device: that call allocates and waits for the copies, on a
+ * stream that is not captured (captures of other streams go on), and dnatok_destroy_grammar may wait for the device; nothing
+ * else waits. */
 
 #define DNATOK_F32  0
 #define DNATOK_F16  1
