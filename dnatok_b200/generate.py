@@ -285,6 +285,12 @@ class Grammar:
         except Exception:
             pass
 
+    def __copy__(self) -> "Grammar":                 # (a grammar does not change, and owns what it would share)
+        return self
+
+    def __deepcopy__(self, memo) -> "Grammar":
+        return self
+
     def start(self, n_rows: int, device=None) -> torch.Tensor:
         """The first state of ``n_rows`` rows."""
         return torch.full((int(n_rows),), self.automaton.start, dtype=torch.int32,
