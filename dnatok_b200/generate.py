@@ -46,12 +46,9 @@ Number = Union[float, int, torch.Tensor]
 _LEAST, _MOST = 2.0 ** -126, 2.0 ** 126              # a repetition penalty whose reciprocal is a normal number too
 
 
-# The open level of forward-mode differentiation, -1 for none (the public ``unpack_dual`` asks for each tensor: 0.5 us apiece).
-def _forward_level() -> int:
-    return getattr(forward_ad, "_current_level", 0)
-
-
-# The current stream of a device as a number (the public call builds a Stream object on the way: 2 us instead of 0.1).
+# The current device, and the current stream of a device, as numbers (the public calls look whether CUDA is up, which it is where
+# there are tensors, and build a Stream object on the way: 0.3 and 2 us instead of 0.1).
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
@@ -75,25 +72,31 @@ def _on(t, what: str, dev: int) -> None:
         raise ValueError("%s is on cuda:%d, the call on cuda:%d" % (what, d, dev))
 
 
-def _address(t: torch.Tensor, what: str) -> int:
-    """Where a tensor's elements are; 0 is no argument to the library, so only a tensor without elements may give it."""
-    p = t.data_ptr()
-    if not p and t.numel():
+def _nowhere(t: torch.Tensor, what: str) -> int:
+    """For ``t.data_ptr() or _nowhere(t, what)``: 0 means an argument that is not there, so only a tensor without elements may
+    have that address."""
+    if t.numel():
         raise ValueError("%s has no memory of its own (a distributed, fake or otherwise wrapped tensor)" % what)
-    return p
+    return 0
+
+
+# make_fx records under a mode for functions; where there is none it need not be asked for (0.05 us instead of 1).
+_modes = getattr(torch._C, "_len_torch_function_stack", None) or (lambda: 1)
+_tracing = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing
 
 
 def _traced() -> bool:
-    """Whether ``torch.jit.trace`` or ``make_fx`` is recording the operations of this thread."""
+    """Whether ``make_fx`` is recording the operations of this thread."""
     proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
-    return torch.jit.is_tracing() or (proxies is not None and proxies.get_proxy_mode() is not None)
+    return proxies is not None and proxies.get_proxy_mode() is not None
 
 
 def _call(fn, dev: int, *args) -> None:
     """A C entry point with the device current and its current stream as the last argument."""
-    if _traced():                                    # (the trace would hold the output's allocation and nothing that fills it)
+    if _tracing() or (_modes() and _traced()):
+        # (the trace would hold the output's allocation and nothing that fills it)
         raise RuntimeError("kernels of this library cannot be recorded by torch.jit.trace or make_fx")
-    if torch.cuda.current_device() == dev:
+    if _current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -107,6 +110,11 @@ def _no_tangents(**named) -> None:
     for name, t in named.items():
         if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError("%s has a tangent; there is no forward-mode derivative" % name)
+
+
+def _no_gradient(name: str, v) -> None:
+    if getattr(v, "requires_grad", False):
+        raise ValueError("%s has no gradient; detach it or call under torch.no_grad()" % name)
 
 
 def _written(t: torch.Tensor) -> None:
@@ -152,7 +160,7 @@ class TokenHistory:
         split = (n_rows * words + 3) // 4 * 4
         both = torch.zeros(split + n_rows * width, dtype=torch.int32, device=device)
         # (.data: views of one array would share its version, and a write to the counts would count as one to the words)
-        return both.as_strided((n_rows, words), (words, 1)).data, both.as_strided((n_rows, width), (width, 1), split).data
+        return both.as_strided((n_rows, words), (words, 1)), both.as_strided((n_rows, width), (width, 1), split).data
 
     @property
     def device(self) -> torch.device:
@@ -194,7 +202,7 @@ class TokenHistory:
             if offsets.dtype is not torch.int64 or offsets.dim() != 1 or offsets.shape[0] < 1 or not offsets.is_contiguous():
                 raise ValueError("offsets must be a contiguous int64 tensor [n + 1]")
             n = offsets.shape[0] - 1
-            h.offsets, h.total = _address(offsets, "offsets"), ids.shape[0]
+            h.offsets, h.total = (offsets.data_ptr() or _nowhere(offsets, "offsets")), ids.shape[0]
         else:
             if ids.dim() != 2 or (ids.shape[1] > 1 and ids.stride(1) != 1):
                 raise ValueError("padded ids must be a tensor [n, T] whose rows are contiguous")
@@ -204,7 +212,7 @@ class TokenHistory:
                 _on(lengths, "lengths", dev)
                 if lengths.dtype is not torch.int32 or lengths.shape != (n,) or not lengths.is_contiguous():
                     raise ValueError("lengths must be a contiguous int32 tensor [%d]" % n)
-                h.lengths = _address(lengths, "lengths")
+                h.lengths = lengths.data_ptr() or _nowhere(lengths, "lengths")
             h.pad_left = 1 if pad_left else 0
         self._enter(h, ids, n, rows, generated, dev)
 
@@ -221,13 +229,13 @@ class TokenHistory:
     def _enter(self, h, ids, n: int, rows, generated: bool, dev: int) -> None:
         if rows is not None:
             h.rows_bits = _tokens(rows, "rows", n, dev)
-            h.rows = _address(rows, "rows")
+            h.rows = rows.data_ptr() or _nowhere(rows, "rows")
         elif n != self.n_rows:
             raise ValueError("the history has %d rows, the call %d" % (self.n_rows, n))
-        h.seen, h.history_rows, h.width = _address(self.seen, "seen"), self.n_rows, self.width
+        h.seen, h.history_rows, h.width = (self.seen.data_ptr() or _nowhere(self.seen, "seen")), self.n_rows, self.width
         if self.counts is not None:
-            h.counts = _address(self.counts, "counts")
-        h.ids, h.id_bits, h.n_rows = _address(ids, "ids"), _BITS[ids.dtype], n
+            h.counts = self.counts.data_ptr() or _nowhere(self.counts, "counts")
+        h.ids, h.id_bits, h.n_rows = (ids.data_ptr() or _nowhere(ids, "ids")), _BITS[ids.dtype], n
         _call(_cabi.lib().dnatok_history_add, dev, h, 1 if generated else 0)
         _written(self.seen)
         if generated and self.counts is not None:
@@ -302,7 +310,7 @@ class Grammar:
         dev = _device_of(states, "states")
         if states.dtype is not torch.int32 or states.dim() != 1 or (states.shape[0] > 1 and states.stride(0) != 1):
             raise ValueError("states must be a contiguous int32 tensor [n]")
-        return states.shape[0], dev, _address(states, "states")
+        return states.shape[0], dev, (states.data_ptr() or _nowhere(states, "states"))
 
     def _mask(self, states, n: int, dev: int, out):
         words = _words(self.width)
@@ -326,7 +334,7 @@ class Grammar:
         """int32 [n, words]: the tokens that may follow in each state."""
         n, dev, at = self._states(states)
         mask = self._mask(states, n, dev, out)
-        _call(_cabi.lib().dnatok_grammar_allowed, dev, self.ptr, at, n, _address(mask, "the mask"))
+        _call(_cabi.lib().dnatok_grammar_allowed, dev, self.ptr, at, n, (mask.data_ptr() or _nowhere(mask, "the mask")))
         if out is not None:
             _written(out)
         return mask
@@ -337,8 +345,8 @@ class Grammar:
         n, dev, at = self._states(states)
         bits = _tokens(tokens, "tokens", n, dev)
         new = self._new_states(states, n, dev, out)
-        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, at, _address(tokens, "tokens"), bits, n,
-              _address(new, "out"), None)
+        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, at, (tokens.data_ptr() or _nowhere(tokens, "tokens")), bits, n,
+              (new.data_ptr() or _nowhere(new, "out")), None)
         if out is not None:
             _written(out)
         return new
@@ -350,8 +358,8 @@ class Grammar:
         bits = _tokens(tokens, "tokens", n, dev)
         new = self._new_states(states, n, dev, out)
         mask = self._mask(states, n, dev, out_allowed)
-        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, at, _address(tokens, "tokens"), bits, n,
-              _address(new, "out"), _address(mask, "the mask"))
+        _call(_cabi.lib().dnatok_grammar_step, dev, self.ptr, at, (tokens.data_ptr() or _nowhere(tokens, "tokens")), bits, n,
+              (new.data_ptr() or _nowhere(new, "out")), (mask.data_ptr() or _nowhere(mask, "the mask")))
         if out is not None:
             _written(out)
         if out_allowed is not None:
@@ -376,7 +384,7 @@ def _penalty(name: str, v, n: int, dev: int):
         _on(v, name, dev)
         if v.dtype is not torch.float32 or v.shape != (n,) or (n > 1 and v.stride(0) != 1):
             raise ValueError("%s must be a number or a contiguous float32 tensor [%d]" % (name, n))
-        return neutral, _address(v, name), True
+        return neutral, (v.data_ptr() or _nowhere(v, name)), True
     v = float(v)
     if neutral:
         if not _LEAST <= v <= _MOST:
@@ -400,10 +408,10 @@ def _row_array(t, what: str, dtype, n: int, columns: int, dev: int) -> Tuple[int
             or (len(shape) == 2 and shape[0] != 1 and shape[0] != n):
         raise ValueError("%s must be a %s tensor [%d, %d] or [%d] whose rows are contiguous" % (what, str(dtype)[6:], n, columns, columns))
     if len(shape) == 1 or shape[0] == 1:
-        return _address(t, what), 0
+        return (t.data_ptr() or _nowhere(t, what)), 0
     if strides[0] < columns:
         raise ValueError("rows of %s overlap" % what)
-    return _address(t, what), strides[0]
+    return (t.data_ptr() or _nowhere(t, what)), strides[0]
 
 
 def _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed):
@@ -414,7 +422,7 @@ def _arguments(logits, history, rows, repetition, frequency, presence, bias, all
     if dtype is None:
         raise ValueError("logits must be float32, float16 or bfloat16")
     a = _cabi.Logits()
-    a.logits, a.dtype, a.n_rows, a.width, a.stride = _address(logits, "logits"), dtype, n, width, stride
+    a.logits, a.dtype, a.n_rows, a.width, a.stride = (logits.data_ptr() or _nowhere(logits, "logits")), dtype, n, width, stride
     a.repetition, a.d_repetition, once = _penalty("repetition", repetition, n, dev)
     a.frequency, a.d_frequency, often = _penalty("frequency", frequency, n, dev)
     a.presence, a.d_presence, also = _penalty("presence", presence, n, dev)
@@ -431,15 +439,15 @@ def _arguments(logits, history, rows, repetition, frequency, presence, bias, all
             raise ValueError("the history is on %s, the logits on %s" % (history.device, logits.device))
         if rows is not None:
             a.rows_bits = _tokens(rows, "rows", n, dev)
-            a.rows = _address(rows, "rows")
+            a.rows = rows.data_ptr() or _nowhere(rows, "rows")
         elif history.n_rows != n:
             raise ValueError("the history has %d rows, the logits %d" % (history.n_rows, n))
         if often and history.counts is None:
             raise ValueError("frequency and presence need a history that keeps counts")
         if once or often:
-            a.seen, a.history_rows = _address(history.seen, "seen"), history.n_rows
+            a.seen, a.history_rows = (history.seen.data_ptr() or _nowhere(history.seen, "seen")), history.n_rows
         if often:
-            a.counts = _address(history.counts, "counts")
+            a.counts = history.counts.data_ptr() or _nowhere(history.counts, "counts")
     if bias is not None:
         a.bias, a.bias_stride = _row_array(bias, "bias", torch.float32, n, width, dev)
     if allowed is not None:
@@ -463,7 +471,7 @@ def _output(logits, out, out_dtype):
 
 
 def _forward(a, dev: int, out):
-    _call(_cabi.lib().dnatok_process_logits, dev, a, _address(out, "out"), _TYPES[out.dtype], out.stride(0))
+    _call(_cabi.lib().dnatok_process_logits, dev, a, (out.data_ptr() or _nowhere(out, "out")), _TYPES[out.dtype], out.stride(0))
     return out
 
 
@@ -472,7 +480,7 @@ def _backward(a, dev: int, dtype, grad, bias_shape, want_logits: bool):
     if grad.shape[1] > 1 and grad.stride(1) != 1:
         grad = grad.contiguous()
     n, width = grad.shape
-    d_grad = _address(grad, "grad")
+    d_grad = grad.data_ptr() or _nowhere(grad, "grad")
     L = _cabi.lib()
     dx = grad.new_empty((n, width), dtype=dtype) if want_logits else None
     db, scratch, need = None, None, 0
@@ -513,16 +521,16 @@ class _Process(torch.autograd.Function):
         a.dtype, a.repetition = _TYPES[ctx.dtype], ctx.number
         a.n_rows, a.width = grad.shape
         if logits is None:
-            a.logits = _address(grad, "grad")        # not read: no token counts as seen
+            a.logits = (grad.data_ptr() or _nowhere(grad, "grad"))        # not read: no token counts as seen
         else:
-            a.logits, a.stride = _address(logits, "logits"), logits.stride(0)
-            a.seen, a.history_rows = _address(seen, "seen"), seen.shape[0]
+            a.logits, a.stride = (logits.data_ptr() or _nowhere(logits, "logits")), logits.stride(0)
+            a.seen, a.history_rows = (seen.data_ptr() or _nowhere(seen, "seen")), seen.shape[0]
             if rows is not None:
-                a.rows, a.rows_bits = _address(rows, "rows"), _BITS[rows.dtype]
+                a.rows, a.rows_bits = (rows.data_ptr() or _nowhere(rows, "rows")), _BITS[rows.dtype]
             if repetition is not None:
-                a.d_repetition = _address(repetition, "repetition")
+                a.d_repetition = repetition.data_ptr() or _nowhere(repetition, "repetition")
         if allowed is not None:
-            a.allowed, a.allowed_stride = _address(allowed, "allowed"), 0 if _shared(allowed.shape) else allowed.stride(0)
+            a.allowed, a.allowed_stride = (allowed.data_ptr() or _nowhere(allowed, "allowed")), 0 if _shared(allowed.shape) else allowed.stride(0)
         dx, db = _backward(a, grad.get_device(), ctx.dtype, grad, ctx.bias_shape if ctx.needs_input_grad[1] else None, ctx.needs_input_grad[0])
         return dx, db, None, None, None, None, None, None, None
 
@@ -543,16 +551,20 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
     All of it is computed in 32 bits and rounded once.  Differentiable in ``logits`` and ``bias`` (a penalty that requires a
     gradient is refused, and so is forward mode); the history and the mask must then stay as they are until the backward pass
     (autograd refuses it otherwise)."""
-    if _forward_level() >= 0:
+    if getattr(forward_ad, "_current_level", 0) >= 0:              # a level is open (to ask every tensor takes 0.5 us apiece)
         _no_tangents(logits=logits, repetition=repetition, frequency=frequency, presence=presence, bias=bias, out=out)
-    recording = torch.is_grad_enabled()
-    if recording:                                    # (here: inside of an autograd function the mode is off)
-        for name, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-            if isinstance(v, torch.Tensor) and v.requires_grad:
-                raise ValueError("%s has no gradient" % name)
-        if getattr(out, "requires_grad", False):
-            raise ValueError("out= has no gradient; leave it out or call under torch.no_grad()")
-    if recording and (getattr(logits, "requires_grad", False) or (bias is not None and getattr(bias, "requires_grad", False))):
+    differentiable = False
+    if torch.is_grad_enabled():                      # (asked here: inside of an autograd function it is not)
+        if repetition.__class__ is not float:
+            _no_gradient("repetition", repetition)
+        if frequency.__class__ is not float:
+            _no_gradient("frequency", frequency)
+        if presence.__class__ is not float:
+            _no_gradient("presence", presence)
+        if out is not None:
+            _no_gradient("out=", out)
+        differentiable = getattr(logits, "requires_grad", False) or (bias is not None and getattr(bias, "requires_grad", False))
+    if differentiable:
         if out is not None:
             raise ValueError("out= has no gradient; leave it out or call under torch.no_grad()")
         return _Process.apply(logits, bias, history, rows, repetition, frequency, presence, allowed, out_dtype)
@@ -567,7 +579,7 @@ def process_logits_backward(grad, logits, *, history: Optional[TokenHistory] = N
                             frequency: Number = 0.0, presence: Number = 0.0, bias=None, allowed=None):
     """(gradient of ``logits``, gradient of ``bias`` or None) for ``grad``, the gradient of ``process_logits`` called with the
     same arguments; without autograd."""
-    if _forward_level() >= 0:
+    if getattr(forward_ad, "_current_level", 0) >= 0:
         _no_tangents(grad=grad, logits=logits, repetition=repetition, frequency=frequency, presence=presence, bias=bias)
     with torch.no_grad():
         a, dev = _arguments(logits, history, rows, repetition, frequency, presence, bias, allowed)

@@ -24,7 +24,7 @@ def library(monkeypatch):
     monkeypatch.setattr(_cabi, "lib", lambda: made)
     monkeypatch.setattr(generate, "_device_of", lambda t, what: t.get_device())
     monkeypatch.setattr(generate, "_raw_stream", lambda index: 0)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)              # the device of a CPU tensor
+    monkeypatch.setattr(generate, "_current_device", lambda: -1)                # the device of a CPU tensor
     return made
 
 
