@@ -170,7 +170,9 @@ dim3 logits_grid(int64_t n_rows, int64_t width, int parts) {
 
 // With a shared bias' gradient a block goes through several groups of rows, as many as leave at most 12 blocks an SM (three
 // whole rounds of 4, four of 3): their partial sums are few beside what they read.  Up to 32 rows one block does them all,
-// four a warp: that takes less than a second launch to join two.
+// four a warp, which saves the launch that joins: about 3 us of the host.  On the GPU alone, calls following one another in a
+// graph, it gains up to 16 rows and loses behind (float, one block and two launches: 16 x 32,000 4.6 and 5.3 us, 9 x 4,096 4.2
+// and 4.6, 32 x 4,096 7.4 and 4.9, 32 x 32,000 10.6 and 6.9).
 dim3 bias_grid(int64_t n_rows, int64_t width, int parts) {
     const int64_t tiles = tiles_of(width, parts);
     int64_t groups = (int64_t)SMS * 12 / tiles;
@@ -223,7 +225,10 @@ int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtyp
     const int parts = logits_parts(a.n_rows, a.width);
     const dim3 grid = logits_grid(a.n_rows, a.width, parts);
     const int64_t logits = (int64_t)a.n_rows * a.width;
-    const bool few = logits <= (int64_t)SMS * 2048;                   // a thread each, all of them on the GPU at once
+    // A thread each, all of them on the GPU at once.  With everything, bf16, a thread a logit and by tiles: 585 x 512 3.2 and 3.2 us,
+    // 1,171 x 512 4.8 and 3.4; 73 x 4,106 3.3 and 3.6, 146 x 4,106 5.0 and 5.8, 292 x 4,106 8.0 and 6.8; 9 x 32,000 3.3 and 3.1 to
+    // 3.8, 18 x 32,000 4.9 and 3.4.  (Rows of few tokens leave most of a tile empty: 120,000 x 10 7.8 and 97.)
+    const bool few = logits <= (int64_t)SMS * 2048;
     with_type(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         auto typed = [&](auto* o) {
@@ -345,12 +350,13 @@ namespace {
 template <typename IdT>
 int launch_history(const HistoryArgs& a, const IdT* ids, cudaStream_t st) {
     const int64_t mean = a.offsets ? a.total / a.n_rows : a.columns;     // ids a row, as far as the host knows
-    // A row with at least as many ids as there are tokens is counted in shared memory first (8 x 1,048,576 ids of bytes:
-    // 10.8 us; entered one by one they queue up at ten counters a row: 10,800 us).  A row that is only marked needs 32
+    // A row with at least as many ids as there are tokens is counted in shared memory first (8 rows of up to 1,048,576 ids of
+    // bytes: 8.1 us; entered one by one they queue up at ten counters a row: 10,800 us).  A row that is only marked needs 32
     // times less to clear and to join.
     const int64_t words = (a.width + 31) / 32, table = a.counts ? a.width : words;
     if (mean >= 1024 && mean >= (a.counts ? table : 4 * table) && table * 4 <= 192 * 1024 && a.n_rows <= (1 << 20)) {
-        // up to 8 counters a token (8 x 1,048,576 ids of bytes: 10.8 us, 12.4 with 32, which take longer to clear and to join)
+        // up to 8 counters a token (these rows: 8.1 us, 8.2 with 32, which take longer to clear and to join, 7.6 with one: ten
+        // tokens in use do not make the lanes of a warp wait for one another as long as one or two would)
         int log_copies = 0;
         while (a.counts && log_copies < 3 && (table << (log_copies + 1)) * 4 <= 48 * 1024) ++log_copies;
         int64_t resident = 220 * 1024 / ((table << log_copies) * 4 + 1024);       // blocks an SM, all of them at once
@@ -518,7 +524,8 @@ int launch_allowed(const GrammarTables& t, const int32_t* states, const void* to
                    uint32_t* allowed, cudaStream_t st) {
     const int64_t words = (t.width + 31) / 32;
     // The groups need a row's words in shared memory, 32 KB beside a small table; vocabularies beyond 262,144 tokens and automata with more than
-    // 15 classes go token by token.
+    // 15 classes go token by token.  (By groups and token by token, motifs to avoid: 64 x 4,106 5.3 and 3.5 us, 1 x 32,000 6.1 and
+    // 3.4, but 1,024 x 4,106 17.6 and 27.5, 64 x 32,000 11.7 and 21.7, 1,024 x 32,000 72 and 312.)
     if (!t.text || words > 8192 || n_rows > INT32_MAX / 8) {
         if (tokens) {
             grammar_advance_kernel<<<(unsigned)((n_rows + GRAMMAR_THREADS - 1) / GRAMMAR_THREADS), GRAMMAR_THREADS, 0, st>>>(

@@ -15,7 +15,7 @@
 // times as many: rows that allow nearly all, which the others wait for, go from 95 to 165 us.)
 //
 // What bounds it: instructions, about 85 a group and warp with its share of everything (1,024 rows of a 2,000-position
-// pattern over 32,000 tokens: 11 M, 29 us, of which the last third is a few rows that allow most tokens), and for few rows
+// pattern over 32,000 tokens: 10.2 M, 29 us, of which the last third is a few rows that allow most tokens), and for few rows
 // the latency of the dependent loads (one row 5 to 6 us).  The bytes are nothing: 4 MB of masks.
 #pragma once
 #include <cooperative_groups.h>

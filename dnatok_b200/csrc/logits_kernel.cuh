@@ -5,8 +5,9 @@
 //   y  = allowed ? x2 + bias : -inf
 //   dx = allowed ? dy (seen ? (x > 0 ? 1 / r : r) : 1) : 0,   dbias = allowed ? dy : 0, over the rows for a shared bias
 //
-// All of it is computed in 32 bits; y and dx are rounded once, to the type of the output.  seen and allowed hold a bit
-// per token (bit v % 32 of word v / 32), so that a count is only read where there is one.
+// All of it is computed in 32 bits, with a rounding an operation (x / r is x * (1 / r): two of them); y and dx are then rounded
+// once, to the type of the output.  seen and allowed hold a bit per token (bit v % 32 of word v / 32), so that a count is only
+// read where a token was seen, and a logit in the backward pass too.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,8 +52,9 @@ __device__ __forceinline__ float of_row(const float* each, float all, int32_t ro
 
 __device__ __forceinline__ bool bit_at(const uint32_t* words, int v) { return __ldg(words + (v >> 5)) >> (v & 31) & 1; }
 
-// Small calls, a thread a logit: nothing is shared, but few instructions stand between the loads (64 rows of 4,106 bf16
-// logits with everything: 4.2 us, the kernel below 6.2).
+// Small calls, a thread a logit: nothing is shared, but few instructions stand between the loads (73 rows of 4,106 bf16
+// logits with everything: 3.3 us, the kernel below 3.6, calls following one another in a graph; the rule and where the two
+// meet stand at the launch).
 template <typename T, typename O>
 __global__ void __launch_bounds__(LOGITS_THREADS)
 process_each_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride) {
@@ -342,7 +344,7 @@ process_logits_kernel(LogitsArgs a, const T* logits, O* out, int64_t out_stride)
 
 // The gradients of the logits at a row's hits, over those of its other allowed tokens.  x: the logit of this lane's first hit,
 // fetched ahead of time.  (By the list, because only there are logits read: among all columns, as the repetition penalty of
-// the forward pass, 2,048 x 32,000 took 119 us instead of 83.)
+// the forward pass, 2,048 x 32,000 took 119 us instead of 83 when that was tried; 74 now, bf16, nine tenths allowed, 5 % seen.)
 template <typename T, typename G>
 __device__ __forceinline__ void mend_gradient(const LogitsArgs& a, int row, int n_hits, const uint16_t* list, T x, const T* x_row, const G* g_row, T* d_row, int lane) {
     __syncwarp();                                             // the order of the stores

@@ -17,7 +17,8 @@ after its chosen token.  A generation loop:
         states, allowed = grammar.step(states, tokens)
 
 Everything numeric happens in ``libdnatok_b200.so``; work is enqueued on the current stream of the tensors' device and
-nothing waits for it.  (``torch.jit.trace`` and ``make_fx`` cannot record that work: the calls refuse to be traced.)
+nothing waits for it, but for a ``Grammar``'s first use on a device, which allocates and uploads its tables.
+(``torch.jit.trace`` and ``make_fx`` cannot record that work: the calls refuse to be traced.)
 Sets of tokens are int32 words: bit ``v % 32`` of word ``v // 32`` stands for token ``v``.
 
 The calls can be captured into a CUDA graph (use a ``Grammar`` on the device once before, and keep it as long as the graph).
@@ -541,16 +542,16 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
     bias and mask, as a new tensor of its type or of ``out_dtype`` float32, or in ``out``, which may be ``logits`` but may
     not overlap them, or another argument, in any other way.
 
-    * A token the row has seen: ``x > 0 ? x / repetition : x * repetition``; one it generated ``c > 0`` times, then
+    * A token the row has seen: ``x > 0 ? x / repetition : x * repetition`` (by the rounded ``1 / repetition``); one it generated ``c > 0`` times, then
       ``- frequency * c - presence``.  Each is a number, or a float32 tensor [n] (repetition from 2^-126 to 2^126 there too).
       ``rows`` [n] names each row's history row (a row outside the history has none); two rows may share one.
     * ``bias`` float32 [width] or [n, width] is added.
     * ``allowed`` int32 [n, words] or [words]: tokens whose bit is 0 become ``-inf`` whatever their logits hold, NaN
       included.  A row without an allowed token is ``-inf`` throughout.
 
-    All of it is computed in 32 bits and rounded once.  Differentiable in ``logits`` and ``bias`` (a penalty that requires a
-    gradient is refused, and so is forward mode); the history and the mask must then stay as they are until the backward pass
-    (autograd refuses it otherwise)."""
+    All of it is computed in 32 bits and then rounded to the output's type.  Differentiable in ``logits`` and ``bias`` (a penalty
+    that requires a gradient is refused, and so is forward mode); the mask and, with a repetition penalty, the logits and the
+    history must then stay as they are until the backward pass (autograd refuses it otherwise)."""
     if getattr(forward_ad, "_current_level", 0) >= 0:              # a level is open (to ask every tensor takes 0.5 us apiece)
         _no_tangents(logits=logits, repetition=repetition, frequency=frequency, presence=presence, bias=bias, out=out)
     differentiable = False

@@ -312,10 +312,10 @@ typedef struct {
 } dnatok_logits;
 
 /* out = allowed ? x2 + bias : -inf, where a token that the row has seen has x1 = x > 0 ? x / repetition : x * repetition
- * (repetition from 2^-126 to 2^126) and one that it generated c > 0 times x2 = x1 - frequency * c - presence; other tokens
- * keep x.  Computed in 32 bits,
- * rounded once to the output's type: that of the logits or DNATOK_F32.  Logits that are not allowed have no influence, NaN
- * included; a row without an allowed token is -inf throughout.  d_out may be the logits themselves (same type and stride);
+ * (repetition from 2^-126 to 2^126; x / repetition is x times the rounded 1 / repetition) and one that it generated c > 0 times
+ * x2 = x1 - frequency * c - presence; other tokens keep x.  Computed in 32 bits, then rounded to the output's type: that of the
+ * logits or DNATOK_F32.  Logits that are not allowed have no influence, NaN included; a row without an allowed token is -inf
+ * throughout.  d_out may be the logits themselves (same type and stride);
  * another overlap, with any array of the call, is refused. */
 int dnatok_process_logits(const dnatok_logits* in, void* d_out, int32_t out_dtype, int64_t out_stride, dnatok_stream stream);
 
