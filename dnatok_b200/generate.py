@@ -522,7 +522,7 @@ class _Process(torch.autograd.Function):
         a.dtype, a.repetition = _TYPES[ctx.dtype], ctx.number
         a.n_rows, a.width = grad.shape
         if logits is None:
-            a.logits = (grad.data_ptr() or _nowhere(grad, "grad"))        # not read: no token counts as seen
+            a.logits = grad.data_ptr() or _nowhere(grad, "grad")          # not read: no token counts as seen
         else:
             a.logits, a.stride = (logits.data_ptr() or _nowhere(logits, "logits")), logits.stride(0)
             a.seen, a.history_rows = (seen.data_ptr() or _nowhere(seen, "seen")), seen.shape[0]
@@ -542,9 +542,10 @@ def process_logits(logits, *, history: Optional[TokenHistory] = None, rows=None,
     bias and mask, as a new tensor of its type or of ``out_dtype`` float32, or in ``out``, which may be ``logits`` but may
     not overlap them, or another argument, in any other way.
 
-    * A token the row has seen: ``x > 0 ? x / repetition : x * repetition`` (by the rounded ``1 / repetition``); one it generated ``c > 0`` times, then
-      ``- frequency * c - presence``.  Each is a number, or a float32 tensor [n] (repetition from 2^-126 to 2^126 there too).
-      ``rows`` [n] names each row's history row (a row outside the history has none); two rows may share one.
+    * A token the row has seen: ``x > 0 ? x / repetition : x * repetition`` (by the rounded ``1 / repetition``); one it
+      generated ``c > 0`` times, then ``- frequency * c - presence``.  Each is a number, or a float32 tensor [n] (repetition
+      from 2^-126 to 2^126 there too).  ``rows`` [n] names each row's history row (a row outside the history has none); two
+      rows may share one.
     * ``bias`` float32 [width] or [n, width] is added.
     * ``allowed`` int32 [n, words] or [words]: tokens whose bit is 0 become ``-inf`` whatever their logits hold, NaN
       included.  A row without an allowed token is ``-inf`` throughout.
